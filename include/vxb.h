@@ -45,6 +45,11 @@ extern "C" {
 #define VXB_TYPE_F32 0
 #define VXB_TYPE_F16 1
 #define VXB_TYPE_Q4_0 2
+/* Types of the language-model operators' tensors: ggml's BF16, and e4m3 codes
+ * (8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448),
+ * which ggml has no number for. */
+#define VXB_TYPE_BF16 30
+#define VXB_TYPE_E4M3 256
 
 typedef struct vxb_ctx vxb_ctx;
 
@@ -305,6 +310,94 @@ VXB_API int vxb_residual_unit(const void* w, int w_type, int C, int d, const flo
  * (src/audio-vae.cpp:1642-1673, :512-534). */
 VXB_API int vxb_convt(const void* w, int w_type, int Cin, int Cout, int s, const void* x_f16, int B, int T,
               const float* bias, float* y, void* stream);
+
+/* ---- language-model operators (device pointers, enqueued on `stream`) ----
+ *
+ * The layer of the speech model that makes the latents vxb_decode_device and
+ * vxb_stream_push_device read (and takes those vxb_encode_device writes), for
+ * callers that run it on the same stream.  No counterpart in the reference,
+ * which holds the codec only.  Strides count elements.  Calls return once
+ * their work is enqueued; every launch is on `stream` of the current device,
+ * allocates nothing and may be captured into a graph.  Work on zero rows is a
+ * success without a launch.  Outputs must not overlap inputs unless said. */
+
+/* Root-mean-square norm of rows, the residual added first:
+ *   h = x (+ residual);  sum = h;  y = h / sqrt(mean(h^2) + eps) * w
+ * x, residual, sum [N][C] of `type` (F32, F16 or BF16), residual and sum may
+ * be NULL, sum may be x or residual; w [C] of `type` or F32.  y is of `type`
+ * (y_scale NULL; y may be x), or with y_type E4M3 codes with y_scale
+ * [N][ceil(C / 128)]: per row and 128 channels scale = max|y| / 448 and code
+ * = e4m3(y / scale), the operand form of vxb_fp8_product (a block whose scale
+ * would be below fp32's normal range is zeros with scale 0).  Sums and the
+ * norm are fp32 of the unrounded h.  1 <= C <= 32768. */
+VXB_API int vxb_rms_norm(int type, int64_t N, int C, const void* x, int64_t x_stride, const void* residual,
+                         int64_t residual_stride, void* sum, int64_t sum_stride, int w_type, const void* w, float eps,
+                         int y_type, void* y, int64_t y_stride, float* y_scale, int64_t scale_stride, void* stream);
+
+/* Product of e4m3 matrices with an fp32 scale for each block of 128:
+ *   y[n][m] = bias[m] + sum_k x[n][k] x_scale[n][k / 128] * w[m][k] w_scale[m / 128][k / 128]
+ * x [N][K], w [M][K] (K contiguous, K % 16 == 0, bases and row strides
+ * multiples of 16 bytes); x_scale [N][ceil(K / 128)] (row stride given),
+ * w_scale [ceil(M / 128)][ceil(K / 128)] contiguous; bias fp32 [M] or NULL;
+ * y [N][M] F32, F16 or BF16.  Products of a block are summed on the tensor
+ * cores, blocks in fp32.  Any N and M, 16 <= K <= 2^24. */
+VXB_API int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x_stride, const float* x_scale,
+                            int64_t x_scale_stride, const void* w, int64_t w_stride, const float* w_scale,
+                            const float* bias, int y_type, void* y, int64_t y_stride, void* stream);
+
+/* Rotary positions: in every head the first R dims (even, <= D, <= 256) turn
+ * in pairs by positions[n] * inv_freq[i] (fp32 [R / 2]), times `factor`; pair
+ * i is dims (i, i + R/2), or (2i, 2i + 1) if interleaved; dims R.. are
+ * copied.  Angles are formed in fp64, so far positions keep their turn.
+ * q [N][Hq][D] -> q_out, and with k given k [N][Hk][D] -> k_out, of `type`
+ * (F32, F16 or BF16) with token and head strides, D contiguous (D <= 1024);
+ * q_out may be q and k_out may be k (same strides). */
+VXB_API int vxb_rotary(int type, int64_t N, int Hq, int Hk, int D, int R, int interleaved, float factor,
+                       const int64_t* positions, const float* inv_freq, const void* q, int64_t q_token,
+                       int64_t q_head, void* q_out, int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
+                       int64_t k_head, void* k_out, int64_t ko_token, int64_t ko_head, void* stream);
+
+/* The same with the rotated keys and the values written to a paged cache:
+ * token n at page slots[n] / page_size, place slots[n] % page_size, of
+ * k_cache and v_cache [pages][page_size][Hk][D] (one set of strides for both,
+ * D contiguous).  A slot outside [0, pages * page_size) -- a padding token's
+ * -- is skipped; its q is still rotated.  Slots within the cache must differ
+ * from one another: which of two tokens with one slot stays is not defined. */
+VXB_API int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R, int interleaved, float factor,
+                              const int64_t* positions, const int64_t* slots, const float* inv_freq, const void* q,
+                              int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token, int64_t qo_head,
+                              const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, void* k_cache, void* v_cache, int64_t pages, int page_size,
+                              int64_t page_stride, int64_t slot_stride, int64_t head_stride, void* stream);
+
+/* Causal attention of B sequences' new tokens over a paged cache that already
+ * holds their keys and values.  Sequence b: rows cu_q[b] .. cu_q[b + 1] of
+ * q [N][Hq][D] and kv_len[b] cached keys, the new tokens' the last of them;
+ * token i stands at p = kv_len - q_len + i and sees keys j <= p, with
+ * window > 0 also j > p - window:
+ *   out = sum_j softmax_j(scale q . k_j) v_j    (zeros if it sees none)
+ * Query head h reads key head h / (Hq / Hk).  Key j lies at page
+ * block_table[b][j / page_size], place j % page_size, of k_cache and v_cache
+ * [pages][page_size][Hk][D] (one set of strides for both).  A table entry
+ * outside [0, pages) makes its keys unseen (a page given back by a sliding
+ * window); entries past a sequence's keys are not read, kv_len beyond
+ * max_pages * page_size is cut to it, and values that no token sees, non-finite
+ * ones too, have no effect.  Rows of q and out outside every sequence are not
+ * touched.  type F16 or BF16; D % 8 == 0, D <= 128; page_size a power of two
+ * >= 16; q and cache bases and strides multiples of 16 bytes.  `workspace`:
+ * vxb_paged_attention_workspace bytes of device memory (0: may be NULL), in
+ * use until the call's work on `stream` is done.  Scores, softmax and sums
+ * are fp32; the weights are rounded to `type` for the second product. */
+VXB_API int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, int D, const void* q, int64_t q_token,
+                                int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages,
+                                int page_size, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                                const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* cu_q,
+                                const int32_t* kv_len, float scale, int window, void* out, int64_t o_token,
+                                int64_t o_head, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that vxb_paged_attention needs for these extents on the
+ * current device; -1 if the extents are refused (vxb_last_error). */
+VXB_API int64_t vxb_paged_attention_workspace(int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size);
 
 #ifdef __cplusplus
 }

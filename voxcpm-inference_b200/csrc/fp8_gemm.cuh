@@ -1,0 +1,350 @@
+// Product of 8-bit (e4m3) matrices with fp32 scales for blocks of 128:
+//
+//   y[n][m] = bias[m] + sum_b xs[n][b] * ws[m / 128][b] * P_b[n][m],
+//   P_b[n][m] = sum_{k in block b} x[n][k] * w[m][k]
+//
+// A scale changes every 128 k, so the tensor cores cannot accumulate over the
+// whole of K: each block's product P_b (four tcgen05.mma of K = 32, kind
+// f8f6f4, fp32 accumulator) goes to one of two TMEM buffers, and the epilogue
+// warps add it, scaled, to the running sum in their registers (fp32) while the
+// next block's product is formed in the other buffer.
+//
+// Two orientations of the 128-row operand (the TMEM lanes):
+//   tokens as rows (many tokens): A = x tile, B = w tile of BN outputs; a
+//     thread holds one token, its x scale is the thread's own and the w scale
+//     is the same for all of a warpgroup's columns: one FMA per element.
+//   weights as rows (few tokens): A = w tile of 128 outputs (one scale block),
+//     B = x tile of BN = 16, 32 or 64 tokens; a thread holds one output, the
+//     w scale is the same for the tile and the x scales of the columns are
+//     kept one per lane and passed around by shuffles.
+// With fewer tiles than SMs, K is split over the blocks of a cluster; each
+// leaves its partial sums in its own shared memory and all of them add a
+// share of the columns over distributed shared memory, in rank order (the
+// result does not depend on timing).
+//
+// Warp roles: warp 0 lane 0 issues TMA loads, warp 1 owns TMEM and issues the
+// MMAs, warps 4.. are one or two epilogue warpgroups (warp w reads TMEM lanes
+// 32 * (w % 4) ..).
+#pragma once
+
+#include <cuda.h>
+
+#include "lm_norm.cuh"
+
+namespace vxb {
+
+enum OutType : int { kOutF32 = 0, kOutF16 = 1, kOutBF16 = 2 };
+
+struct Fp8GemmArgs {
+    int64_t N;                 // tokens
+    int K, M;                  // inner extent, outputs
+    int kb;                    // blocks of 128 k
+    int row_tiles;             // tiles along the 128-row operand
+    int64_t tiles;             // row_tiles * column tiles
+    const float* xs;           // [N][kb], row stride xs_stride
+    int64_t xs_stride;
+    const float* ws;           // [ceil(M / 128)][kb]
+    const float* bias;         // [M] or null
+    void* y;                   // [N][M], row stride y_stride
+    int64_t y_stride;
+    int out_type;
+    int split;                 // blocks of a cluster that share a tile's K
+};
+
+// Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3 (format 0), dense, both K-major.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
+    return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Issues the load of 16 TMEM columns without waiting for it.
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void cluster_arrive_wait() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
+    float v;
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}\n"
+                 : "=f"(v)
+                 : "r"(saddr), "r"(rank)
+                 : "memory");
+    return v;
+}
+
+template <int BN, bool WROWS>
+struct Fp8Cfg {
+    static constexpr int kGroups = BN > 64 ? 2 : 1;     // epilogue warpgroups
+    static constexpr int kCols = BN / kGroups;          // columns of a warpgroup
+    static constexpr int kThreads = 128 + 128 * kGroups;
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = BN * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStagesFit = (224 * 1024 - 2048) / kStageBytes;
+    static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
+    static constexpr int kBufCols = BN < 32 ? 32 : BN;
+    static constexpr int kTmemCols = 2 * kBufCols;
+    static constexpr int kRedBytes = BN * 128 * 4;      // split: partial sums [BN][128], over the stages
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+    static_assert(kRedBytes <= kStages * kStageBytes, "partial sums fit the drained stages");
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+    static_assert(BN % 16 == 0 && BN <= 256, "UMMA N");
+    static_assert(!WROWS || kGroups == 1, "weights as rows: at most 64 tokens wide");
+};
+
+__device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type) {
+    if (type == kOutF32) {
+        static_cast<float*>(y)[i] = v;
+    } else if (type == kOutF16) {
+        static_cast<__half*>(y)[i] = __float2half_rn(v);
+    } else {
+        static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+    }
+}
+
+template <int BN, bool WROWS>
+__global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const Fp8GemmArgs args) {
+    using Cfg = Fp8Cfg<BN, WROWS>;
+    constexpr int S = Cfg::kStages;
+    constexpr int NC = Cfg::kCols;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(stages + S * Cfg::kStageBytes);
+    uint64_t* empty_bar = full_bar + S;
+    uint64_t* tfull_bar = empty_bar + S;   // product [2] complete
+    uint64_t* tempty_bar = tfull_bar + 2;  // product [2] read
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int split = args.split;
+    const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    // this block's share of the k blocks
+    const int kb_lo = static_cast<int>(static_cast<int64_t>(args.kb) * rank / split);
+    const int kb_hi = static_cast<int>(static_cast<int64_t>(args.kb) * (rank + 1) / split);
+    const int64_t tile0 = blockIdx.x / split;
+    const int64_t tile_step = gridDim.x / split;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full_bar[i], 1);
+            mbar_init(&empty_bar[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull_bar[i], 1);
+            mbar_init(&tempty_bar[i], 4 * Cfg::kGroups);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmap_a);
+        prefetch_tmap(&tmap_b);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    grid_dep_sync();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------------------------------------- TMA producer --
+            int it = 0;
+            for (int64_t tile = tile0; tile < args.tiles && !*abort_flag; tile += tile_step) {
+                const int r0 = static_cast<int>(tile % args.row_tiles) * 128;
+                const int c0 = static_cast<int>(tile / args.row_tiles) * BN;
+                for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+                    const int st = it % S;
+                    if (!mbar_wait(&empty_bar[st], ((it / S) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty)) break;
+                    uint8_t* dst = stages + st * Cfg::kStageBytes;
+                    mbar_arrive_expect_tx(&full_bar[st], Cfg::kStageBytes);
+                    tma_load_2d(dst, &tmap_a, &full_bar[st], kb * 128, r0);
+                    tma_load_2d(dst + Cfg::kABytes, &tmap_b, &full_bar[st], kb * 128, c0);
+                }
+            }
+            if (*abort_flag) {  // give copies already in flight time to land
+                const unsigned long long t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 1000000ull) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ----------------------------------------------- MMA issuer --
+            constexpr uint32_t idesc = make_idesc_e4m3(128, BN);
+            int it = 0;
+            bool ok = true;
+            for (int64_t tile = tile0; tile < args.tiles && ok; tile += tile_step) {
+                for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+                    const int st = it % S, buf = it & 1;
+                    if (!mbar_wait(&tempty_bar[buf], ((it >> 1) & 1) ^ 1, abort_flag, nullptr, kErrWaitAccum) ||
+                        !mbar_wait(&full_bar[st], (it / S) & 1, abort_flag, nullptr, kErrWaitFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(stages + st * Cfg::kStageBytes);
+                    const uint32_t b_addr = a_addr + Cfg::kABytes;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)  // K = 32 bytes per instruction inside the 128-byte rows
+                        umma_f8(tmem_base + buf * Cfg::kBufCols, make_sdesc(a_addr + kk * 32, 16, 1024),
+                                make_sdesc(b_addr + kk * 32, 16, 1024), idesc, kk != 0);
+                    umma_commit(&empty_bar[st]);
+                    umma_commit(&tfull_bar[buf]);
+                }
+            }
+            if (!ok) {  // completes once every issued MMA is done: TMEM and the stages are idle after it
+                umma_commit(&tfull_bar[0]);
+                umma_commit(&tfull_bar[1]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ---------------------------------------------------- epilogue --
+        const int eg = (warp - 4) >> 2;
+        const int q = warp & 3;
+        const int row = q * 32 + lane;
+        const uint32_t t_row = tmem_base + eg * NC + (static_cast<uint32_t>(q * 32) << 16);
+        int it = 0;
+        for (int64_t tile = tile0; tile < args.tiles; tile += tile_step) {
+            const int r = static_cast<int>(tile % args.row_tiles) * 128 + row;   // A row of this thread
+            const int c0 = static_cast<int>(tile / args.row_tiles) * BN + eg * NC;  // first column of this group
+            // scales: `own` of the thread's row, `col` of the columns (tokens as rows: one for
+            // all of them; weights as rows: lane l keeps columns l and l + 32)
+            const float *own_p, *col_p, *col_p2 = nullptr;
+            if (WROWS) {
+                own_p = args.ws + static_cast<int64_t>(r / 128) * args.kb;
+                col_p = c0 + lane < args.N && lane < BN ? args.xs + (c0 + lane) * args.xs_stride : nullptr;
+                col_p2 = BN > 32 && c0 + 32 + lane < args.N ? args.xs + (c0 + 32 + lane) * args.xs_stride : nullptr;
+            } else {
+                own_p = r < args.N ? args.xs + r * args.xs_stride : nullptr;
+                col_p = c0 < args.M ? args.ws + static_cast<int64_t>(c0 / 128) * args.kb : nullptr;
+            }
+            float acc[NC];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) acc[i] = 0.f;
+            auto load = [](const float* p, int kb) { return p ? __ldg(p + kb) : 0.f; };
+            float own = 0.f, col = 0.f, col2 = 0.f;
+            if (kb_lo < kb_hi) own = load(own_p, kb_lo), col = load(col_p, kb_lo), col2 = load(col_p2, kb_lo);
+            bool ok = true;
+            for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+                const int buf = it & 1;
+                float own_n = 0.f, col_n = 0.f, col2_n = 0.f;
+                if (kb + 1 < kb_hi) {  // the next block's scales
+                    own_n = load(own_p, kb + 1);
+                    col_n = load(col_p, kb + 1);
+                    col2_n = load(col_p2, kb + 1);
+                }
+                ok = mbar_wait(&tfull_bar[buf], (it >> 1) & 1, abort_flag, nullptr, kErrWaitAccum);
+                ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t t = t_row + buf * Cfg::kBufCols;
+                constexpr int CH = NC < 32 ? NC : 32;  // columns in flight
+                const float s = own * col;
+#pragma unroll
+                for (int c = 0; c < NC; c += CH) {
+                    uint32_t v[CH];
+#pragma unroll
+                    for (int i = 0; i < CH; i += 16) tmem_ld16_async(t + c + i, v + i);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < CH; i += 2) {
+                        float2 sc = make_float2(s, s);
+                        if (WROWS) {
+                            const float from = c + i < 32 ? col : col2;
+                            sc.x = own * __shfl_sync(0xffffffffu, from, (c + i) & 31);
+                            sc.y = own * __shfl_sync(0xffffffffu, from, (c + i + 1) & 31);
+                        }
+                        const float2 p = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        const float2 o = ffma2(sc, p, make_float2(acc[c + i], acc[c + i + 1]));
+                        acc[c + i] = o.x;
+                        acc[c + i + 1] = o.y;
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tempty_bar[buf]);
+                own = own_n;
+                col = col_n;
+                col2 = col2_n;
+            }
+            if (!ok) break;
+            if (split > 1) {
+                // partial sums [column][row] over the drained stages (one tile per cluster)
+                float* red = reinterpret_cast<float*>(stages);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) red[(eg * NC + i) * 128 + row] = acc[i];
+                break;
+            }
+            if (WROWS) {
+                const float b = args.bias && r < args.M ? args.bias[r] : 0.f;
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+                    if (r < args.M && c0 + i < args.N)
+                        store_out(args.y, (c0 + i) * args.y_stride + r, acc[i] + b, args.out_type);
+            } else if (r < args.N) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+                    if (c0 + i < args.M)
+                        store_out(args.y, r * args.y_stride + c0 + i, acc[i] + (args.bias ? args.bias[c0 + i] : 0.f),
+                                  args.out_type);
+            }
+        }
+    }
+
+    if (split > 1) {
+        __syncwarp();
+        cluster_arrive_wait();  // every rank's partial sums are written
+        if (!*abort_flag && tile0 < args.tiles) {
+            const int r0 = static_cast<int>(tile0 % args.row_tiles) * 128;
+            const int64_t c0 = tile0 / args.row_tiles * BN;
+            const uint32_t red = smem_u32(stages);
+            // rank's share: columns rank, rank + split, ...; a warp's lanes are neighbours along
+            // the output's fast axis (weights as rows: rows; tokens as rows: columns are the fast
+            // axis of y, rows are read for coalesced shared memory)
+            for (int i = rank * static_cast<int>(blockDim.x) + threadIdx.x; i < BN * 128; i += split * blockDim.x) {
+                const int c = i >> 7, rr = i & 127;
+                const int64_t n = WROWS ? c0 + c : r0 + rr;
+                const int64_t m = WROWS ? r0 + rr : c0 + c;
+                if (n >= args.N || m >= args.M) continue;
+                float v = 0.f;
+                for (int p = 0; p < split; ++p) v += ld_cluster_f32(red + i * 4, p);
+                if (args.bias) v += args.bias[m];
+                store_out(args.y, n * args.y_stride + m, v, args.out_type);
+            }
+        }
+        __syncwarp();
+        cluster_arrive_wait();  // no rank leaves while its shared memory is read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+}
+
+}  // namespace vxb

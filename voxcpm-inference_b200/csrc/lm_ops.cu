@@ -1,0 +1,418 @@
+// Language-model operators of the C ABI: RMS norm with 8-bit output, 8-bit
+// block-scaled product, rotary positions into a paged cache, attention over
+// a paged cache.  Arguments are checked before any CUDA call; every entry
+// point only enqueues work on `stream`.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "fp8_gemm.cuh"
+#include "host.h"
+#include "lm_norm.cuh"
+#include "lm_rotary.cuh"
+#include "paged_attn.cuh"
+#include "vxb.h"
+
+using namespace vxb;
+
+namespace {
+
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024;  // rows addressed by 32-bit tile coordinates
+
+int bad(const char* op, const char* what) {
+    return fail(VXB_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what);
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int elem_size(int type) { return type == VXB_TYPE_F32 ? 4 : 2; }
+
+bool is_float(int type) { return type == VXB_TYPE_F32 || type == VXB_TYPE_F16 || type == VXB_TYPE_BF16; }
+
+int this_device(int* dev) {
+    CUDA_TRY(cudaGetDevice(dev));
+    return VXB_OK;
+}
+
+// No C++ exception leaves the C ABI.
+template <typename F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return VXB_ERR_OUT_OF_MEMORY;
+    } catch (...) {
+        return VXB_ERR_BACKEND;
+    }
+}
+
+// ---------------------------------------------------------------- rms norm --
+
+template <typename T, int NV>
+cudaError_t launch_norm_v(const NormArgs& a, bool vec, int threads, cudaStream_t st) {
+    const dim3 g(static_cast<unsigned>(a.N)), b(threads);
+    return vec ? launch_pdl(rms_norm_kernel<T, NV, true>, g, b, 0, st, a)
+               : launch_pdl(rms_norm_kernel<T, NV, false>, g, b, 0, st, a);
+}
+
+template <typename T>
+cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
+    const int vecs = (a.C + 7) / 8;
+    const auto threads = [&](int nv) { return std::max(32, (vecs + 32 * nv - 1) / (32 * nv) * 32); };
+    if (threads(1) <= 256) return launch_norm_v<T, 1>(a, vec, threads(1), st);
+    if (threads(2) <= 1024) return launch_norm_v<T, 2>(a, vec, threads(2), st);
+    return launch_norm_v<T, 4>(a, vec, threads(4), st);
+}
+
+}  // namespace
+
+extern "C" int vxb_rms_norm(int type, int64_t N, int C, const void* x, int64_t x_stride, const void* residual,
+                            int64_t residual_stride, void* sum, int64_t sum_stride, int w_type, const void* w,
+                            float eps, int y_type, void* y, int64_t y_stride, float* y_scale, int64_t scale_stride,
+                            void* stream) {
+    const char* op = "rms_norm";
+    return guarded([&]() -> int {
+        if (!is_float(type)) return bad(op, "x must be f32, f16 or bf16");
+        if (w_type != type && w_type != VXB_TYPE_F32) return bad(op, "the weight must be of x's type or f32");
+        if (y_type != type && y_type != VXB_TYPE_E4M3) return bad(op, "the output must be of x's type or e4m3");
+        if (N < 0 || N > kMaxRows) return bad(op, "bad row count");
+        if (C < 1 || C > 32768) return bad(op, "width must be 1..32768");
+        if (!(eps >= 0.f) || std::isinf(eps)) return bad(op, "eps must be finite and not negative");
+        const bool q8 = y_type == VXB_TYPE_E4M3;
+        if (N == 0) return VXB_OK;
+        if (!x || !w || !y) return bad(op, "null argument");
+        if (q8 != (y_scale != nullptr)) return bad(op, "e4m3 output takes a scale, other outputs none");
+        if (x_stride < C || y_stride < C || (residual && residual_stride < C) || (sum && sum_stride < C) ||
+            (q8 && scale_stride < (C + kScaleBlock - 1) / kScaleBlock))
+            return bad(op, "a row stride is smaller than the row");
+        const int es = elem_size(type);
+        if (!aligned(x, es) || !aligned(residual, es) || !aligned(sum, es) || !aligned(w, elem_size(w_type)) ||
+            !aligned(y, q8 ? 1 : es) || !aligned(y_scale, 4))
+            return bad(op, "a pointer is not aligned to its element");
+        NormArgs a{x,  residual, sum, w,        y,        y_scale,      N, x_stride, residual_stride, sum_stride,
+                   y_stride, scale_stride, C, w_type == VXB_TYPE_F32 && type != VXB_TYPE_F32, eps};
+        const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(y, q8 ? 8 : 16) && aligned(residual, 16) &&
+                         aligned(sum, 16) && x_stride % 8 == 0 && y_stride % 8 == 0 &&
+                         (!residual || residual_stride % 8 == 0) && (!sum || sum_stride % 8 == 0);
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        CUDA_TRY(type == VXB_TYPE_F32   ? launch_norm<float>(a, vec, st)
+                 : type == VXB_TYPE_F16 ? launch_norm<__half>(a, vec, st)
+                                        : launch_norm<__nv_bfloat16>(a, vec, st));
+        return VXB_OK;
+    });
+}
+
+// ------------------------------------------------------------------ rotary --
+
+namespace {
+
+template <typename T, int VEC>
+cudaError_t launch_rotary(const RotaryArgs& a, bool inter, cudaStream_t st) {
+    const dim3 g(static_cast<unsigned>((a.N + a.tokens - 1) / a.tokens)), b(kRotThreads);
+    return inter ? launch_pdl(rotary_kernel<T, VEC, true>, g, b, 0, st, a)
+                 : launch_pdl(rotary_kernel<T, VEC, false>, g, b, 0, st, a);
+}
+
+bool head_vec(const void* p, int64_t token, int64_t head, int vec) {
+    return !p || (aligned(p, 16) && token % vec == 0 && head % vec == 0);
+}
+
+int run_rotary(const char* op, int type, RotaryArgs a, int interleaved, void* stream) {
+    if (!is_float(type)) return bad(op, "the type must be f32, f16 or bf16");
+    if (a.N < 0 || a.N > kMaxRows) return bad(op, "bad token count");
+    if (a.Hq < 1 || a.Hk < 0 || a.Hq > 65535 || a.Hk > 65535) return bad(op, "bad head count");
+    if (a.D < 1 || a.D > 1024) return bad(op, "head width must be 1..1024");
+    if (a.R < 2 || a.R % 2 || a.R > a.D || a.R > kRotMaxR)
+        return bad(op, "the rotated part must be even, at most the head and at most 256");
+    if (std::isnan(a.factor) || std::isinf(a.factor)) return bad(op, "the factor must be finite");
+    if (a.N == 0) return VXB_OK;
+    if (!a.q.p || !a.q_out.p || !a.positions || !a.inv_freq) return bad(op, "null argument");
+    const int es = elem_size(type);
+    for (const void* p : {static_cast<const void*>(a.q.p), static_cast<const void*>(a.q_out.p),
+                          static_cast<const void*>(a.k.p), static_cast<const void*>(a.k_out.p),
+                          static_cast<const void*>(a.v.p), static_cast<const void*>(a.k_cache),
+                          static_cast<const void*>(a.v_cache)})
+        if (!aligned(p, es)) return bad(op, "a pointer is not aligned to its element");
+    if (!aligned(a.positions, 8) || !aligned(a.slots, 8) || !aligned(a.inv_freq, 4))
+        return bad(op, "positions, slots or frequencies are not aligned to their elements");
+    const int vec = 16 / es;
+    const bool v = a.D % vec == 0 && a.R % (2 * vec) == 0 && head_vec(a.q.p, a.q.token, a.q.head, vec) &&
+                   head_vec(a.q_out.p, a.q_out.token, a.q_out.head, vec) &&
+                   head_vec(a.k.p, a.k.token, a.k.head, vec) &&
+                   head_vec(a.k_out.p, a.k_out.token, a.k_out.head, vec) &&
+                   head_vec(a.v.p, a.v.token, a.v.head, vec) &&
+                   head_vec(a.k_cache, a.page_stride, a.slot_stride, vec) &&
+                   head_vec(a.v_cache, a.page_stride, a.cache_head, vec);
+    int dev = 0, rc = this_device(&dev);
+    if (rc) return rc;
+    a.tokens = static_cast<int>(std::min<int64_t>(kRotTokens, std::max<int64_t>(1, a.N / (4 * num_sms(dev)))));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (type == VXB_TYPE_F32) {
+        CUDA_TRY(v ? (launch_rotary<float, 4>(a, interleaved, st)) : (launch_rotary<float, 1>(a, interleaved, st)));
+    } else if (type == VXB_TYPE_F16) {
+        CUDA_TRY(v ? (launch_rotary<__half, 8>(a, interleaved, st)) : (launch_rotary<__half, 1>(a, interleaved, st)));
+    } else {
+        CUDA_TRY(v ? (launch_rotary<__nv_bfloat16, 8>(a, interleaved, st))
+                   : (launch_rotary<__nv_bfloat16, 1>(a, interleaved, st)));
+    }
+    return VXB_OK;
+}
+
+}  // namespace
+
+extern "C" int vxb_rotary(int type, int64_t N, int Hq, int Hk, int D, int R, int interleaved, float factor,
+                          const int64_t* positions, const float* inv_freq, const void* q, int64_t q_token,
+                          int64_t q_head, void* q_out, int64_t qo_token, int64_t qo_head, const void* k,
+                          int64_t k_token, int64_t k_head, void* k_out, int64_t ko_token, int64_t ko_head,
+                          void* stream) {
+    return guarded([&]() -> int {
+        if ((k != nullptr) != (k_out != nullptr)) return bad("rotary", "keys and their output come together");
+        if (k && Hk < 1 && N > 0) return bad("rotary", "bad head count");
+        RotaryArgs a{};
+        a.q = {const_cast<void*>(q), q_token, q_head};
+        a.q_out = {q_out, qo_token, qo_head};
+        a.k = {const_cast<void*>(k), k_token, k_head};
+        a.k_out = {k_out, ko_token, ko_head};
+        a.positions = positions;
+        a.inv_freq = inv_freq;
+        a.page_size = 1;
+        a.N = N, a.Hq = Hq, a.Hk = Hk, a.D = D, a.R = R, a.factor = factor;
+        return run_rotary("rotary", type, a, interleaved, stream);
+    });
+}
+
+extern "C" int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R, int interleaved, float factor,
+                                 const int64_t* positions, const int64_t* slots, const float* inv_freq,
+                                 const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
+                                 int64_t qo_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                                 int64_t v_token, int64_t v_head, void* k_cache, void* v_cache, int64_t pages,
+                                 int page_size, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                                 void* stream) {
+    const char* op = "rotary_append";
+    return guarded([&]() -> int {
+        if (pages < 0 || page_size < 1 || pages > (int64_t(1) << 40) / page_size) return bad(op, "bad cache extents");
+        if (Hk < 1) return bad(op, "bad head count");
+        if (N > 0 && (!k || !v || !slots || !k_cache || !v_cache)) return bad(op, "null argument");
+        RotaryArgs a{};
+        a.q = {const_cast<void*>(q), q_token, q_head};
+        a.q_out = {q_out, qo_token, qo_head};
+        a.k = {const_cast<void*>(k), k_token, k_head};
+        a.v = {const_cast<void*>(v), v_token, v_head};
+        a.positions = positions;
+        a.inv_freq = inv_freq;
+        a.slots = slots;
+        a.k_cache = k_cache;
+        a.v_cache = v_cache;
+        a.cache_slots = pages * page_size;
+        a.page_stride = page_stride, a.slot_stride = slot_stride, a.cache_head = head_stride;
+        a.page_size = page_size;
+        a.N = N, a.Hq = Hq, a.Hk = Hk, a.D = D, a.R = R, a.factor = factor;
+        return run_rotary(op, type, a, interleaved, stream);
+    });
+}
+
+// ------------------------------------------------------------- fp8 product --
+
+namespace {
+
+// e4m3 matrix [rows][K] (row pitch in bytes), boxes of 128 k x box_rows.
+int make_tmap_e4m3(CUtensorMap* m, const void* base, uint64_t K, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {K, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled (e4m3) failed: " + std::to_string(r));
+    return VXB_OK;
+}
+
+struct Fp8Operands {
+    const void *x, *w;
+    int64_t x_stride, w_stride;
+};
+
+template <int BN, bool WROWS>
+int launch_fp8(const Fp8Operands& o, Fp8GemmArgs a, int dev, cudaStream_t st) {
+    using Cfg = Fp8Cfg<BN, WROWS>;
+    static std::atomic<bool> attr[64];
+    int rc = allow_smem(fp8_gemm_kernel<BN, WROWS>, Cfg::kSmemBytes, attr, dev);
+    if (rc) return rc;
+    const int64_t rows = WROWS ? a.M : a.N, cols = WROWS ? a.N : a.M;
+    a.row_tiles = static_cast<int>((rows + 127) / 128);
+    a.tiles = a.row_tiles * ((cols + BN - 1) / BN);
+    // fewer tiles than SMs: K is shared by the blocks of a cluster, each with two k blocks at least
+    const int sms = num_sms(dev);
+    a.split = 1;
+    while (a.split < 8 && a.tiles * a.split * 2 <= sms && a.kb >= a.split * 4) a.split *= 2;
+    CUtensorMap tx, tw;
+    if ((rc = make_tmap_e4m3(&tx, o.x, a.K, a.N, o.x_stride, WROWS ? BN : 128))) return rc;
+    if ((rc = make_tmap_e4m3(&tw, o.w, a.K, a.M, o.w_stride, WROWS ? 128 : BN))) return rc;
+    const int64_t grid = a.split > 1 ? a.tiles * a.split : std::min<int64_t>(a.tiles, sms);
+    CUDA_TRY(launch_pdl_cluster(fp8_gemm_kernel<BN, WROWS>, dim3(static_cast<unsigned>(grid)), dim3(Cfg::kThreads),
+                                a.split, Cfg::kSmemBytes, st, WROWS ? tw : tx, WROWS ? tx : tw, a));
+    return VXB_OK;
+}
+
+}  // namespace
+
+extern "C" int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x_stride, const float* x_scale,
+                               int64_t x_scale_stride, const void* w, int64_t w_stride, const float* w_scale,
+                               const float* bias, int y_type, void* y, int64_t y_stride, void* stream) {
+    const char* op = "fp8_product";
+    return guarded([&]() -> int {
+        if (N < 0 || N > kMaxRows) return bad(op, "bad row count");
+        if (K < 16 || K % 16 || K > (1 << 24)) return bad(op, "K must be a multiple of 16");
+        if (M < 1 || M > (1 << 30)) return bad(op, "bad output width");
+        if (!is_float(y_type)) return bad(op, "the output must be f32, f16 or bf16");
+        if (N == 0) return VXB_OK;
+        if (!x || !x_scale || !w || !w_scale || !y) return bad(op, "null argument");
+        const int kb = (K + kScaleBlock - 1) / kScaleBlock;
+        if (x_stride < K || w_stride < K || y_stride < M || x_scale_stride < kb)
+            return bad(op, "a row stride is smaller than the row");
+        if (!aligned(x, 16) || !aligned(w, 16) || x_stride % 16 || w_stride % 16)
+            return bad(op, "TMA operand needs 16-byte aligned base and row pitch");
+        if (!aligned(x_scale, 4) || !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(y, elem_size(y_type)))
+            return bad(op, "a pointer is not aligned to its element");
+        int dev = 0, rc = this_device(&dev);
+        if (rc) return rc;
+        Fp8GemmArgs a{};
+        a.N = N, a.K = K, a.M = M, a.kb = kb;
+        a.xs = x_scale, a.xs_stride = x_scale_stride, a.ws = w_scale, a.bias = bias;
+        a.y = y, a.y_stride = y_stride;
+        a.out_type = y_type == VXB_TYPE_F32 ? kOutF32 : y_type == VXB_TYPE_F16 ? kOutF16 : kOutBF16;
+        const Fp8Operands o{x, w, x_stride, w_stride};
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (N <= 16) return launch_fp8<16, true>(o, a, dev, st);
+        if (N <= 32) return launch_fp8<32, true>(o, a, dev, st);
+        if (N <= 64) return launch_fp8<64, true>(o, a, dev, st);
+        if ((N + 127) / 128 * ((M + 255) / 256) >= num_sms(dev)) return launch_fp8<256, false>(o, a, dev, st);
+        return launch_fp8<128, false>(o, a, dev, st);
+    });
+}
+
+// --------------------------------------------------------- paged attention --
+
+namespace {
+
+constexpr int kAttnMaxD = 128;
+
+// How many parts a call's keys are split into: as many as fill the device
+// with two blocks per SM, no part shorter than 256 keys of a full table.
+int attn_splits(int64_t blocks, int64_t max_keys, int sms) {
+    const int64_t want = 2 * int64_t(sms) / std::max<int64_t>(1, blocks);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_keys / 256, 64})));
+}
+
+int64_t attn_blocks(int64_t N, int B, int Hk, int G, int rows) {
+    const int TT = std::max(1, rows / G), GT = std::min(G, rows);
+    return (N / TT + B) * Hk * ((G + GT - 1) / GT);
+}
+
+int attn_rows(int64_t N, int B, int G) { return N * G > int64_t(B) * 16 ? 32 : 16; }
+
+template <typename T, int DP, int MT>
+int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
+    using Cfg = AttnCfg<T, DP, MT>;
+    static std::atomic<bool> attr[64];
+    int rc = allow_smem(attn_rows_kernel<T, DP, MT>, Cfg::kSmemBytes, attr, dev);
+    if (rc) return rc;
+    const int TT = std::max(1, Cfg::kRows / a.G), GT = std::min(a.G, Cfg::kRows);
+    const dim3 g(static_cast<unsigned>(a.N / TT + a.B), static_cast<unsigned>(a.Hk * ((a.G + GT - 1) / GT)),
+                 static_cast<unsigned>(a.splits));
+    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, a));
+    if (a.splits > 1)
+        CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>((a.N * a.Hq + 3) / 4)), dim3(128), 0, st,
+                            a));
+    return VXB_OK;
+}
+
+template <typename T>
+int launch_attn_t(const AttnArgs& a, int rows, int dev, cudaStream_t st) {
+    if (a.D <= 64) return rows == 16 ? launch_attn<T, 64, 1>(a, dev, st) : launch_attn<T, 64, 2>(a, dev, st);
+    return rows == 16 ? launch_attn<T, 128, 1>(a, dev, st) : launch_attn<T, 128, 2>(a, dev, st);
+}
+
+int check_attn(const char* op, int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size) {
+    if (N < 0 || N > kMaxRows || B < 0 || B > (1 << 24)) return bad(op, "bad token or sequence count");
+    if (Hk < 1 || Hq < 1 || Hq % Hk || Hq > 4096) return bad(op, "query heads must be a multiple of key heads");
+    if (D < 8 || D % 8 || D > kAttnMaxD) return bad(op, "head width must be a multiple of 8, 8..128");
+    if (page_size < 16 || (page_size & (page_size - 1)) || page_size > (1 << 20))
+        return bad(op, "page size must be a power of two, 16 at least");
+    if (max_pages < 0 || int64_t(max_pages) * page_size >= (int64_t(1) << 31) - 4096)
+        return bad(op, "a table row must cover less than 2^31 keys");
+    return VXB_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t vxb_paged_attention_workspace(int64_t N, int B, int Hq, int Hk, int D, int max_pages,
+                                                 int page_size) {
+    return guarded([&]() -> int { return check_attn("paged_attention", N, B, Hq, Hk, D, max_pages, page_size); })
+               ? -1
+               : [&]() -> int64_t {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return -1;
+        const int G = Hq / Hk, rows = attn_rows(N, B, G);
+        const int splits = attn_splits(attn_blocks(N, B, Hk, G, rows), int64_t(max_pages) * page_size, num_sms(dev));
+        return splits > 1 ? int64_t(splits) * N * Hq * (D + 1) * 4 : 0;
+    }();
+}
+
+extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, int D, const void* q, int64_t q_token,
+                                   int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages,
+                                   int page_size, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                                   const int32_t* block_table, int64_t table_stride, int max_pages,
+                                   const int32_t* cu_q, const int32_t* kv_len, float scale, int window, void* out,
+                                   int64_t o_token, int64_t o_head, void* workspace, int64_t workspace_bytes,
+                                   void* stream) {
+    const char* op = "paged_attention";
+    return guarded([&]() -> int {
+        int rc = check_attn(op, N, B, Hq, Hk, D, max_pages, page_size);
+        if (rc) return rc;
+        if (type != VXB_TYPE_F16 && type != VXB_TYPE_BF16) return bad(op, "the type must be f16 or bf16");
+        if (pages < 0) return bad(op, "bad page count");
+        if (window < 0) return bad(op, "the window must not be negative");
+        if (std::isnan(scale) || std::isinf(scale)) return bad(op, "the scale must be finite");
+        if (N == 0 || B == 0) return VXB_OK;
+        if (!q || !out || !cu_q || !kv_len) return bad(op, "null argument");
+        if (max_pages > 0 && (!block_table || (pages > 0 && (!k_cache || !v_cache))))
+            return bad(op, "null argument");
+        if (max_pages > 0 && B > 1 && table_stride < max_pages) return bad(op, "a table row overlaps the next");
+        if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || q_token % 8 || q_head % 8 ||
+            page_stride % 8 || slot_stride % 8 || head_stride % 8)
+            return bad(op, "queries and cache need 16-byte aligned bases and strides");
+        if (!aligned(out, 2) || !aligned(block_table, 4) || !aligned(cu_q, 4) || !aligned(kv_len, 4))
+            return bad(op, "a pointer is not aligned to its element");
+        int dev = 0;
+        if ((rc = this_device(&dev))) return rc;
+        AttnArgs a{};
+        a.q = q, a.q_token = q_token, a.q_head = q_head;
+        a.out = out, a.o_token = o_token, a.o_head = o_head;
+        a.k = k_cache ? k_cache : q, a.v = v_cache ? v_cache : q;  // (pages = 0: addresses only, nothing is read)
+        a.page_stride = page_stride, a.slot_stride = slot_stride, a.cache_head = head_stride;
+        a.table = block_table, a.table_stride = table_stride, a.cu_q = cu_q, a.kv_len = kv_len;
+        a.N = N, a.pages = k_cache ? pages : 0, a.B = B, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk, a.D = D;
+        a.page_size = page_size, a.max_pages = max_pages, a.window = window;
+        while ((1 << a.page_shift) < page_size) ++a.page_shift;
+        a.scale_log2 = scale * 1.4426950408889634f;
+        const int rows = attn_rows(N, B, a.G);
+        a.splits = attn_splits(attn_blocks(N, B, Hk, a.G, rows), int64_t(max_pages) * page_size, num_sms(dev));
+        if (a.splits > 1) {
+            const int64_t need = int64_t(a.splits) * N * Hq * (D + 1) * 4;
+            if (!workspace || workspace_bytes < need || !aligned(workspace, 4))
+                return bad(op, "the workspace is smaller than vxb_paged_attention_workspace says");
+            a.part_o = static_cast<float*>(workspace);
+            a.part_lse = a.part_o + int64_t(a.splits) * N * Hq * D;
+        }
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        return type == VXB_TYPE_F16 ? launch_attn_t<__half>(a, rows, dev, st)
+                                    : launch_attn_t<__nv_bfloat16>(a, rows, dev, st);
+    });
+}

@@ -1,0 +1,481 @@
+// Attention of new tokens over a paged cache, few query rows at a time.
+//
+// For sequence b with q_len new tokens and kv_len cached keys (the new ones
+// included), token i stands at position p = kv_len - q_len + i and sees the
+// keys j with j <= p and (window > 0) j > p - window:
+//   out = sum_j softmax_j(scale * q . k_j) v_j, zeros if it sees none.
+// Key j lies in page table[b][j / page_size], place j % page_size.  A table
+// entry outside [0, pages) makes its keys unseen.
+//
+// The G = Hq / Hk query heads that share a key head are rows of one tile
+// (row = token * G + head), so a key is read once for all of them: with one
+// new token per sequence the kernel reads K and V once and is HBM bound.  A
+// block has 4 warps and one tile of 16 * MT rows; a step is 64 keys, of which
+// each warp takes 16: it keeps its own running maximum, sum and output
+// (mma.sync m16n8k16, fp32), so no warp waits for another's softmax, and the
+// four are joined once at the end.  The tensor work of a few rows is far
+// below the time of its bytes, so the accumulators stay in registers and the
+// loads are plain 16-byte cp.async through a ring of kStages steps.
+//
+// With few (sequence, head) pairs the keys are split over blockIdx.z; each
+// part leaves its normalised output and log2 of its sum (fp32), and
+// attn_join_kernel weighs them.
+//
+// exp(s * scale - max) is computed as exp2 of s * scale * log2(e) - max.  P is
+// rounded to the cache's type for the second product (at most half a step,
+// 2^-9 of each weight in bf16), the sum is taken of the unrounded weights.
+#pragma once
+
+#include "lm_norm.cuh"
+
+namespace vxb {
+
+constexpr int kAttnStep = 64;      // keys per step
+constexpr int kAttnThreads = 128;
+constexpr float kNegInf = -INFINITY;
+
+struct AttnArgs {
+    const void* q;
+    int64_t q_token, q_head;       // strides in elements
+    void* out;
+    int64_t o_token, o_head;
+    const void* k;
+    const void* v;
+    int64_t page_stride, slot_stride, cache_head;
+    const int* table;              // [B][table_stride]
+    int64_t table_stride;
+    const int* cu_q;               // [B + 1]
+    const int* kv_len;             // [B]
+    int64_t N;                     // rows of q
+    int64_t pages;
+    int B, Hq, Hk, G, D;
+    int page_size, page_shift;
+    int max_pages;                 // entries of a table row
+    int window;
+    float scale_log2;              // softmax scale * log2(e)
+    int splits;
+    float* part_o;                 // [splits][N * Hq][D]
+    float* part_lse;               // [splits][N * Hq], log2 of the sum, -inf if empty
+};
+
+template <typename T>
+struct MmaType;
+template <>
+struct MmaType<__half> {
+    static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+};
+template <>
+struct MmaType<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// A tile of query rows: which sequence, its tokens and keys.
+struct AttnTile {
+    int b;            // -1: nothing to do
+    int tok0;         // first token of the tile within the sequence
+    int q0;           // the sequence's first row of q
+    int q_len, kv_len;
+};
+
+// Tile slots of TT tokens are numbered so that sequence b starts at slot
+// cu_q[b] / TT + b: the next sequence's start is at least ceil(q_len / TT)
+// later, so every tile has a slot and a slot finds its sequence from cu_q
+// alone, with no sum over the sequences before it.  Lengths out of range (the
+// table's capacity, the rows of q) are cut.  All threads call it.
+__device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int64_t slot, int TT, AttnTile* sh) {
+    if (threadIdx.x == 0) sh->b = -1;
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+        const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+        const int kv = a.kv_len[b];
+        if (lo < 0 || hi <= lo || hi > a.N) continue;
+        const int64_t base = lo / TT + b;
+        const int64_t t0 = (slot - base) * TT;
+        if (slot >= base && t0 < hi - lo) {
+            const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page_size;
+            sh->b = b;
+            sh->tok0 = static_cast<int>(t0);
+            sh->q0 = lo;
+            sh->q_len = hi - lo;
+            sh->kv_len = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kv), cap)));
+        }
+    }
+    __syncthreads();
+    return *sh;
+}
+
+template <typename T, int DP, int MT>
+struct AttnCfg {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kRowBytes = DP * 2;
+    static constexpr int kTileBytes = kAttnStep * kRowBytes;   // K or V of one step
+    static constexpr int kStages = DP > 64 ? 3 : 4;
+    static constexpr int kQBytes = kRows * kRowBytes;
+    static constexpr int kSmemBytes = kStages * 2 * kTileBytes + kQBytes;
+    static constexpr int kJoinBytes = 4 * kRows * DP * 4 + 4 * kRows * 8;  // reuses the ring
+    static_assert(kJoinBytes <= kStages * 2 * kTileBytes, "the joining fits the ring");
+};
+
+// Byte offset of 16-byte chunk c of row r in a tile of DP-wide 16-bit rows
+// (chunk index XOR row: ldmatrix reads of 8 rows hit all banks).
+template <int DP>
+__device__ __forceinline__ uint32_t attn_off(int r, int c) {
+    return static_cast<uint32_t>(r * DP * 2 + ((c ^ (r & 7)) << 4));
+}
+
+// Sum of the non-finite values of v[.., d] over the keys [j0, j1) of sequence
+// row `table`: 0 if there are none.
+template <typename T>
+__device__ float attn_poison(const AttnArgs& a, const int* table, int head, int d, int j0, int j1) {
+    float s = 0.f;
+    for (int j = j0; j < j1; ++j) {
+        const int pg = table[j / a.page_size];
+        if (pg < 0 || pg >= a.pages) continue;
+        const float v = to_float(static_cast<const T*>(a.v)[pg * a.page_stride + (j % a.page_size) * a.slot_stride +
+                                                            head * a.cache_head + d]);
+        if (!isfinite(v)) s += v;
+    }
+    return s;
+}
+
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs a) {
+    using Cfg = AttnCfg<T, DP, MT>;
+    using Mma = MmaType<T>;
+    constexpr int S = Cfg::kStages;
+    constexpr int CH = DP / 8;  // 16-byte chunks of a row
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* sq = smem + S * 2 * Cfg::kTileBytes;
+    __shared__ AttnTile sh_tile;
+    __shared__ int sh_poison;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int TT = Cfg::kRows / a.G > 0 ? Cfg::kRows / a.G : 1;  // tokens per tile
+    const int GT = min(a.G, Cfg::kRows);                         // heads of the group per tile
+    const int gparts = (a.G + GT - 1) / GT;                      // tiles a group of heads takes
+    const int hk = blockIdx.y / gparts;
+    const int g0 = (blockIdx.y % gparts) * GT;
+    if (tid == 0) sh_poison = 0;
+    grid_dep_sync();
+    const AttnTile t = find_tile(a, blockIdx.x, TT, &sh_tile);
+    if (t.b < 0) return;
+    const int toks = min(TT, t.q_len - t.tok0);
+    const int heads = min(GT, a.G - g0);
+    // row r of the tile: token r / GT, head r % GT
+    const int pos0 = t.kv_len - t.q_len + t.tok0;  // position of the tile's first token (may be negative)
+    const int* table = a.table + t.b * a.table_stride;
+
+    // keys any row sees, and this part's share of them in whole steps
+    const int key_hi = min(t.kv_len, pos0 + toks);
+    int key_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+    const int step_lo = key_lo / kAttnStep;
+    const int step_hi = key_hi > key_lo ? (key_hi + kAttnStep - 1) / kAttnStep : step_lo;
+    const int64_t steps = step_hi - step_lo;
+    const int my_lo = step_lo + static_cast<int>(steps * blockIdx.z / a.splits);
+    const int my_hi = step_lo + static_cast<int>(steps * (blockIdx.z + 1) / a.splits);
+
+    // queries: rows of the tile (zeros past the tokens and past D)
+    for (int i = tid; i < Cfg::kRows * CH; i += kAttnThreads) {
+        const int r = i / CH, c = i % CH;
+        const int tk = r / GT, g = r % GT;
+        const bool on = tk < toks && g < heads && c * 8 < a.D;
+        const T* src = static_cast<const T*>(a.q);
+        if (on) src += (static_cast<int64_t>(t.q0) + t.tok0 + tk) * a.q_token + (hk * a.G + g0 + g) * a.q_head + c * 8;
+        cp_async16(sq + attn_off<DP>(r, c), src, on ? 16 : 0);
+    }
+    auto load_step = [&](int step) {
+        uint8_t* dk = smem + ((step - my_lo) % S) * 2 * Cfg::kTileBytes;
+        uint8_t* dv = dk + Cfg::kTileBytes;
+#pragma unroll 4
+        for (int i = tid; i < kAttnStep * CH; i += kAttnThreads) {
+            const int r = i / CH, c = i % CH;
+            const int j = step * kAttnStep + r;
+            const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
+            const bool on = pg >= 0 && pg < a.pages && c * 8 < a.D;
+            const int64_t off = on ? pg * a.page_stride + (j & (a.page_size - 1)) * a.slot_stride +
+                                         hk * a.cache_head + c * 8
+                                   : 0;
+            cp_async16(dk + attn_off<DP>(r, c), static_cast<const T*>(a.k) + off, on ? 16 : 0);
+            cp_async16(dv + attn_off<DP>(r, c), static_cast<const T*>(a.v) + off, on ? 16 : 0);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+        if (my_lo + s < my_hi) load_step(my_lo + s);
+        asm volatile("cp.async.commit_group;" ::: "memory");  // (the queries go with the first group)
+    }
+
+    float o[MT][DP / 8][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+        m[i][0] = m[i][1] = kNegInf;
+        l[i][0] = l[i][1] = 0.f;
+    }
+    // the position of each of this thread's rows (row lane/4 and lane/4 + 8 of each m16)
+    int pos[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = i * 16 + h * 8 + (lane >> 2);
+            pos[i][h] = r / GT < toks && r % GT < heads ? pos0 + r / GT : -1;
+        }
+    const int pos_min = pos0, pos_max = pos0 + toks - 1;
+    bool poison = false;
+
+    for (int step = my_lo; step < my_hi; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncthreads();  // the step has landed, and every warp is done with the buffer loaded next
+        if (step + S - 1 < my_hi) load_step(step + S - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+
+        uint8_t* bk = smem + ((step - my_lo) % S) * 2 * Cfg::kTileBytes;
+        uint8_t* bv = bk + Cfg::kTileBytes;
+        const int j0 = step * kAttnStep + warp * 16;  // this warp's keys
+        // does every row see all of the warp's keys?
+        bool whole = j0 + 15 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
+        uint32_t absent = 0;  // bit i: key j0 + i lies in no page
+        {
+            const int j = j0 + (lane & 15);
+            const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
+            absent = __ballot_sync(0xffffffffu, pg < 0 || pg >= a.pages) & 0xffffu;
+            whole = whole && absent == 0;
+        }
+        if (!whole) {
+            // A key that some row does not see has weight 0 there, but 0 * inf is NaN: non-finite
+            // values leave the tile and are added at the end to the rows that see them.
+            for (int i = lane; i < 16 * CH; i += 32) {
+                const int r = warp * 16 + i / CH, c = i % CH;
+                uint4* p = reinterpret_cast<uint4*>(bv + attn_off<DP>(r, c));
+                uint4 raw = *p;
+                T* e = reinterpret_cast<T*>(&raw);
+                bool bad = false;
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if (!isfinite(to_float(e[x]))) {
+                        bad = true;
+                        e[x] = from_float<T>(0.f);
+                    }
+                if (bad) {
+                    poison = true;
+                    *p = raw;
+                }
+            }
+            __syncwarp();
+        }
+
+        // S = Q K^T of 16 * MT rows x 16 keys
+        float s[MT][2][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t kb[4];
+            // matrices: keys 0-7 and 8-15, each k halves 0-7, 8-15
+            ldsm_x4(kb, smem_u32(bk) + attn_off<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                uint32_t qa[4];
+                ldsm_x4(qa, smem_u32(sq) + attn_off<DP>(i * 16 + (lane & 15), 2 * k + (lane >> 4)));
+                Mma::mma(s[i][0], qa, kb[0], kb[1]);
+                Mma::mma(s[i][1], qa, kb[2], kb[3]);
+            }
+        }
+        uint32_t pa[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = kNegInf;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v = s[i][n][2 * h + e] * a.scale_log2;
+                        if (!whole) {
+                            const int kk = n * 8 + (lane & 3) * 2 + e;
+                            const int j = j0 + kk;
+                            if (j > pos[i][h] || (a.window > 0 && j <= pos[i][h] - a.window) || ((absent >> kk) & 1))
+                                v = kNegInf;
+                        }
+                        s[i][n][2 * h + e] = v;
+                        // (a NaN score has to reach the sum: max ignores it)
+                        top = fmaxf(top, v);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m[i][h], top);
+                const float base = mn == kNegInf ? 0.f : mn;
+                const float corr = exp2f(m[i][h] - base);
+                m[i][h] = mn;
+                float sum = 0.f;
+                float p[2][2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        p[n][e] = exp2f(s[i][n][2 * h + e] - base);
+                        sum += p[n][e];
+                    }
+                l[i][h] = l[i][h] * corr + sum;
+                pa[i][h] = Mma::pack(p[0][0], p[0][1]);
+                pa[i][2 + h] = Mma::pack(p[1][0], p[1][1]);
+#pragma unroll
+                for (int j = 0; j < DP / 8; ++j) {
+                    o[i][j][2 * h] *= corr;
+                    o[i][j][2 * h + 1] *= corr;
+                }
+            }
+        }
+        // O += P V
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+            uint32_t vb[4];
+            // matrices: (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (keys 0-7, dims 8-15), (8-15, 8-15)
+            ldsm_x4_t(vb, smem_u32(bv) + attn_off<DP>(warp * 16 + (lane & 15), 2 * d + (lane >> 4)));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                Mma::mma(o[i][2 * d], pa[i], vb[0], vb[1]);
+                Mma::mma(o[i][2 * d + 1], pa[i], vb[2], vb[3]);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (poison) sh_poison = 1;
+    __syncthreads();
+
+    // Join the four warps: each leaves its output, maximum and sum.
+    float* jo = reinterpret_cast<float*>(smem);                  // [4][rows][DP]
+    float* jm = jo + 4 * Cfg::kRows * DP;                        // [4][rows]
+    float* jl = jm + 4 * Cfg::kRows;                             // [4][rows]
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = i * 16 + h * 8 + (lane >> 2);
+            float sum = l[i][h];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if ((lane & 3) == 0) {
+                jm[warp * Cfg::kRows + r] = m[i][h];
+                jl[warp * Cfg::kRows + r] = sum;
+            }
+#pragma unroll
+            for (int j = 0; j < DP / 8; ++j)
+                *reinterpret_cast<float2*>(&jo[(warp * Cfg::kRows + r) * DP + j * 8 + (lane & 3) * 2]) =
+                    make_float2(o[i][j][2 * h], o[i][j][2 * h + 1]);
+        }
+    __syncthreads();
+    for (int i = tid; i < Cfg::kRows * DP; i += kAttnThreads) {
+        const int r = i / DP, d = i % DP;
+        const int tk = r / GT, g = r % GT;
+        if (tk >= toks || g >= heads || d >= a.D) continue;
+        float top = kNegInf;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, jm[w * Cfg::kRows + r]);
+        const float base = top == kNegInf ? 0.f : top;
+        float sum = 0.f, val = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2f(jm[w * Cfg::kRows + r] - base);
+            sum += f * jl[w * Cfg::kRows + r];
+            val += f * jo[(w * Cfg::kRows + r) * DP + d];
+        }
+        // (an empty row has sum 0; a NaN score makes the sum NaN)
+        float y = sum == 0.f ? 0.f : val / sum;
+        if (sh_poison) {
+            const int p = pos0 + tk;
+            const int lo = max(my_lo * kAttnStep, a.window > 0 ? max(0, p - a.window + 1) : 0);
+            const int hi = min(my_hi * kAttnStep, min(p + 1, t.kv_len));
+            y += attn_poison<T>(a, table, hk, d, lo, hi);
+        }
+        const int64_t tok = static_cast<int64_t>(t.q0) + t.tok0 + tk;
+        const int head = hk * a.G + g0 + g;
+        if (a.splits == 1) {
+            static_cast<T*>(a.out)[tok * a.o_token + head * a.o_head + d] = from_float<T>(y);
+        } else {
+            const int64_t row = (blockIdx.z * a.N + tok) * a.Hq + head;
+            a.part_o[row * a.D + d] = y;
+            if (d == 0) a.part_lse[row] = sum == 0.f ? kNegInf : base + log2f(sum);
+        }
+    }
+}
+
+// out[row] = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max); a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+    grid_dep_sync();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= a.N * a.Hq) return;
+    const int64_t tok = row / a.Hq;
+    const int head = static_cast<int>(row % a.Hq);
+    // rows outside every sequence are left as they are
+    bool in = false;
+    for (int b = lane; b < a.B; b += 32) {
+        const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+        in = in || (lo >= 0 && hi <= a.N && tok >= lo && tok < hi);
+    }
+    if (!__any_sync(0xffffffffu, in)) return;
+    float top = kNegInf;
+    bool nan = false;
+    for (int s = 0; s < a.splits; ++s) {
+        const float v = a.part_lse[s * a.N * a.Hq + row];
+        nan = nan || v != v;
+        top = fmaxf(top, v);
+    }
+    const float base = top == kNegInf ? 0.f : top;
+    float sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) sum += exp2f(a.part_lse[s * a.N * a.Hq + row] - base);
+    for (int d = lane; d < a.D; d += 32) {
+        float v = 0.f;
+        for (int s = 0; s < a.splits; ++s) {
+            const float w = exp2f(a.part_lse[s * a.N * a.Hq + row] - base);
+            if (w != 0.f) v += w * a.part_o[(s * a.N * a.Hq + row) * a.D + d];
+        }
+        const float y = sum == 0.f ? 0.f : v / sum;
+        static_cast<T*>(a.out)[tok * a.o_token + head * a.o_head + d] = from_float<T>(nan ? NAN : y);
+    }
+}
+
+}  // namespace vxb

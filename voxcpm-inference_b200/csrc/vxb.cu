@@ -25,34 +25,21 @@
 #include "resunit.cuh"
 #include "convt_tm.cuh"
 #include "gguf_reader.h"
+#include "host.h"
 #include "vxb.h"
 
 using namespace vxb;
 
-// ------------------------------------------------------------------ errors --
+// ------------------------------------------------------------ host helpers --
 
-namespace {
+namespace vxb {
 
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int fail(int code, const std::string& msg) {
     g_last_error = msg;
     return code;
 }
-
-#define CUDA_TRY(expr)                                                                              \
-    do {                                                                                            \
-        cudaError_t e_ = (expr);                                                                    \
-        if (e_ != cudaSuccess)                                                                      \
-            return fail(e_ == cudaErrorMemoryAllocation ? VXB_ERR_OUT_OF_MEMORY : VXB_ERR_BACKEND, \
-                        std::string(#expr) + ": " + cudaGetErrorString(e_));                       \
-    } while (0)
-
-// --------------------------------------------------------------- tensor maps --
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
     static EncodeTiledFn fn = nullptr;
@@ -65,6 +52,23 @@ EncodeTiledFn encode_fn() {
     }
     return fn;
 }
+
+int num_sms(int dev) {
+    static int cache[64] = {};
+    if (dev < 0 || dev >= 64) return 148;
+    if (!cache[dev]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        cache[dev] = n;
+    }
+    return cache[dev];
+}
+
+}  // namespace vxb
+
+// --------------------------------------------------------------- tensor maps --
+
+namespace {
 
 // 2-D fp16 tensor [outer][inner] (inner contiguous) with a {box_inner, box_outer}
 // box and the 128-byte swizzle; out-of-range elements read as zero.
@@ -139,17 +143,6 @@ int make_tmap_u8(CUtensorMap* m, const void* base, uint64_t pitch, uint64_t rows
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled (u8) failed: " + std::to_string(r));
     return VXB_OK;
-}
-
-int num_sms(int dev) {
-    static int cache[64] = {};
-    if (dev < 0 || dev >= 64) return 148;
-    if (!cache[dev]) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-        cache[dev] = n;
-    }
-    return cache[dev];
 }
 
 // A conv weight as a GEMM operand: fp16 bytes, or Q4_0 blocks split into
@@ -273,26 +266,6 @@ int fill_bn(int bn, int m_tiles, int64_t N, int overlap) {
     const int64_t sms = num_sms(dev);
     while (bn > 32 && int64_t(m_tiles) * ((N + bn - overlap - 1) / (bn - overlap)) < sms) bn /= 2;
     return bn;
-}
-
-// Launches a decode kernel with programmatic stream serialisation (the
-// kernel calls grid_dep_sync before it touches activations), so its launch
-// and setup overlap the previous kernel; captured into graphs as
-// programmatic edges.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 template <int AK, int BN, int EPI, int RESKB = 0>

@@ -28,9 +28,11 @@ ERR_DEVICE_STATUS = 8
 ERR_MISSING_TENSOR = 9
 
 TYPE_F32, TYPE_F16, TYPE_Q4_0 = 0, 1, 2
+TYPE_BF16, TYPE_E4M3 = 30, 256
 
 # Every exported symbol of include/vxb.h with its ctypes signature.
 _vp, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_f = ctypes.c_float
 SIGNATURES = {
     "vxb_last_error": (ctypes.c_char_p, []),
     "vxb_open": (_i, [_i, ctypes.POINTER(_vp)]),
@@ -73,6 +75,14 @@ SIGNATURES = {
     "vxb_encode_op_info": (_i, [_vp, _i, ctypes.c_char_p, _i, ctypes.c_char_p, _i, ctypes.POINTER(ctypes.c_double),
                                 ctypes.POINTER(ctypes.c_double)]),
     "vxb_encode_time_ops": (_i, [_vp, _i, _vp, _sz, ctypes.POINTER(ctypes.c_float)]),
+    "vxb_rms_norm": (_i, [_i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _f, _i, _vp, _i64, _vp, _i64, _vp]),
+    "vxb_fp8_product": (_i, [_i64, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i64, _vp]),
+    "vxb_rotary": (_i, [_i, _i64, _i, _i, _i, _i, _i, _f, _vp, _vp] + [_vp, _i64, _i64] * 4 + [_vp]),
+    "vxb_rotary_append": (_i, [_i, _i64, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp] + [_vp, _i64, _i64] * 4
+                          + [_vp, _vp, _i64, _i, _i64, _i64, _i64, _vp]),
+    "vxb_paged_attention": (_i, [_i, _i64, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _vp,
+                                 _i64, _i, _vp, _vp, _f, _i, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "vxb_paged_attention_workspace": (_i64, [_i64, _i, _i, _i, _i, _i, _i]),
 }
 
 
@@ -483,3 +493,229 @@ def residual_unit(w, w_type: int, C: int, d: int, x, batch: int, T: int, a1, dw,
                   out_f16: bool = False, stream=None):
     check(lib().vxb_residual_unit(ptr(w), w_type, C, d, ptr(x), batch, T, ptr(a1), ptr(dw), ptr(db), ptr(a2), ptr(pb),
                                   ptr(out_alpha), 1 if out_f16 else 0, ptr(y), _stream(stream)))
+
+
+# ------------------------------------------------- language-model operators --
+# Tensors on one CUDA device, outputs given by the caller; sizes and strides
+# are the tensors' own (the last axis contiguous).  Work is enqueued on
+# `stream` or the device's current stream, on the tensors' device whichever
+# device is current.  A call that the C ABI or these checks refuse raises
+# VxbError(ERR_INVALID_ARGUMENT) and enqueues nothing.
+
+_types: dict = {}
+
+
+def _type_of(t) -> int:
+    if not _types:
+        import torch
+
+        _types.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16,
+                       torch.float8_e4m3fn: TYPE_E4M3})
+    return _types.get(t.dtype, -1)
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise VxbError(ERR_INVALID_ARGUMENT, what)
+
+
+def _rows(t, what: str, *shape):
+    """Checks a tensor's shape (None: any extent) and that its last axis is contiguous."""
+    _need(t.dim() == len(shape) and all(s is None or n == s for n, s in zip(t.shape, shape)),
+          f"{what}: expected shape {list(shape)}, got {list(t.shape)}")
+    _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{what}: the last axis must be contiguous")
+
+
+def _call(name: str, args, tensors, stream):
+    """Calls a C entry on the tensors' device and stream (appended to args)."""
+    import torch
+
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None:
+            _need(t.device == dev and t.is_cuda, f"{name}: tensors must be on one CUDA device")
+    fn = getattr(lib(), "vxb_" + name)
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, _stream(stream)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(stream)))
+
+
+def rms_norm(x, weight, y, y_scale=None, residual=None, sum_out=None, eps: float = 1e-6, stream=None):
+    """RMS norm of the rows of x [N, C] (float32, float16 or bfloat16), `residual`
+    added first; the sum goes to `sum_out` (may be x or residual).  y: of x's
+    type, or float8_e4m3fn with y_scale float32 [N, ceil(C / 128)]."""
+    _rows(x, "x", None, None)
+    N, C = x.shape
+    _rows(weight, "weight", C)
+    _rows(y, "y", N, C)
+    for t, what in ((residual, "residual"), (sum_out, "sum_out")):
+        if t is not None:
+            _rows(t, what, N, C)
+            _need(t.dtype == x.dtype, f"{what}: must be of x's type")
+    if y_scale is not None:
+        _rows(y_scale, "y_scale", N, -(-C // 128))
+        _need(_type_of(y_scale) == TYPE_F32, "y_scale: must be float32")
+    rs = (lambda t: 0 if t is None else C if N == 1 else t.stride(0))
+    _call("rms_norm", (_type_of(x), N, C, ptr(x), rs(x), ptr(residual), rs(residual), ptr(sum_out), rs(sum_out),
+                       _type_of(weight), ptr(weight), eps, _type_of(y), ptr(y), rs(y), ptr(y_scale),
+                       0 if y_scale is None else -(-C // 128) if N == 1 else y_scale.stride(0)),
+          (x, weight, y, y_scale, residual, sum_out), stream)
+
+
+def fp8_product(x, x_scale, w, w_scale, y, bias=None, stream=None):
+    """y [N, M] = (x * x_scale) @ (w * w_scale)^T + bias for float8_e4m3fn x [N, K]
+    and w [M, K], x_scale float32 [N, ceil(K / 128)] (one per token and block of
+    128), w_scale float32 [ceil(M / 128), ceil(K / 128)], bias float32 [M]."""
+    _rows(x, "x", None, None)
+    N, K = x.shape
+    _rows(w, "w", None, K)
+    M = w.shape[0]
+    kb = -(-K // 128)
+    _rows(x_scale, "x_scale", N, kb)
+    _rows(w_scale, "w_scale", -(-M // 128), kb)
+    _rows(y, "y", N, M)
+    _need(_type_of(x) == TYPE_E4M3 and _type_of(w) == TYPE_E4M3, "x and w must be float8_e4m3fn")
+    _need(_type_of(x_scale) == TYPE_F32 and _type_of(w_scale) == TYPE_F32, "the scales must be float32")
+    _need(w_scale.is_contiguous(), "w_scale must be contiguous")
+    if bias is not None:
+        _rows(bias, "bias", M)
+        _need(_type_of(bias) == TYPE_F32, "bias must be float32")
+    _call("fp8_product", (N, K, M, ptr(x), x.stride(0) if N > 1 else -(-K // 16) * 16, ptr(x_scale),
+                          x_scale.stride(0) if N > 1 else kb, ptr(w), w.stride(0) if M > 1 else -(-K // 16) * 16,
+                          ptr(w_scale), ptr(bias), _type_of(y), ptr(y), y.stride(0) if N > 1 else M),
+          (x, x_scale, w, w_scale, y, bias), stream)
+
+
+def _heads(t, what: str, N, H, D, dtype):
+    _rows(t, what, N, H, D)
+    _need(t.dtype == dtype, f"{what}: must be of q's type")
+    return ptr(t), t.stride(0), t.stride(1)
+
+
+def _angles(positions, inv_freq, N):
+    import torch
+
+    _rows(positions, "positions", N)
+    _need(positions.dtype == torch.int64, "positions must be int64")
+    _rows(inv_freq, "inv_freq", None)
+    _need(_type_of(inv_freq) == TYPE_F32, "inv_freq must be float32")
+    return 2 * inv_freq.shape[0]
+
+
+def rotary(q, positions, inv_freq, q_out, k=None, k_out=None, interleaved: bool = False, factor: float = 1.0,
+           stream=None):
+    """Rotates the first 2 * len(inv_freq) dims of every head of q [N, Hq, D] (and k
+    [N, Hk, D]) by positions [N] (int64) times inv_freq (float32), times
+    `factor`, into q_out (and k_out); q_out may be q, k_out k."""
+    _rows(q, "q", None, None, None)
+    N, Hq, D = q.shape
+    R = _angles(positions, inv_freq, N)
+    Hk = 0
+    _need((k is None) == (k_out is None), "k and k_out come together")
+    if k is not None:
+        _rows(k, "k", N, None, D)
+        Hk = k.shape[1]
+    none = (None, 0, 0)
+    _call("rotary", (_type_of(q), N, Hq, Hk, D, R, 1 if interleaved else 0, factor, ptr(positions), ptr(inv_freq),
+                     *_heads(q, "q", N, Hq, D, q.dtype), *_heads(q_out, "q_out", N, Hq, D, q.dtype),
+                     *(none if k is None else _heads(k, "k", N, Hk, D, q.dtype)),
+                     *(none if k is None else _heads(k_out, "k_out", N, Hk, D, q.dtype))),
+          (q, positions, inv_freq, q_out, k, k_out), stream)
+
+
+def _cache(k_cache, v_cache, Hk, D, dtype):
+    _rows(k_cache, "k_cache", None, None, Hk, D)
+    _need(v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride(),
+          "k_cache and v_cache must have one shape and one set of strides")
+    _need(k_cache.dtype == dtype and v_cache.dtype == dtype, "the cache must be of q's type")
+    return k_cache.shape[0], k_cache.shape[1], k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
+
+
+def rotary_append(q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache, interleaved: bool = False,
+                  factor: float = 1.0, stream=None):
+    """rotary() with the rotated keys and the values [N, Hk, D] written to the paged
+    caches [pages, page_size, Hk, D] at slots [N] (int64; page * page_size +
+    place, each its own; outside the cache: skipped)."""
+    import torch
+
+    _rows(q, "q", None, None, None)
+    N, Hq, D = q.shape
+    R = _angles(positions, inv_freq, N)
+    _rows(slots, "slots", N)
+    _need(slots.dtype == torch.int64, "slots must be int64")
+    _rows(k, "k", N, None, D)
+    Hk = k.shape[1]
+    _call("rotary_append", (_type_of(q), N, Hq, Hk, D, R, 1 if interleaved else 0, factor, ptr(positions), ptr(slots),
+                            ptr(inv_freq), *_heads(q, "q", N, Hq, D, q.dtype),
+                            *_heads(q_out, "q_out", N, Hq, D, q.dtype), *_heads(k, "k", N, Hk, D, q.dtype),
+                            *_heads(v, "v", N, Hk, D, q.dtype), ptr(k_cache), ptr(v_cache),
+                            *_cache(k_cache, v_cache, Hk, D, q.dtype)),
+          (q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache), stream)
+
+
+def rotary_frequencies(R: int, base: float = 10000.0, linear: float = 1.0, factors=None, original_length: int = 0,
+                       length: int = 0):
+    """(inv_freq float32 [R / 2], factor) for rotary(): base^(-2i / R), scaled for
+    contexts longer than a model was trained on.  `linear` divides every
+    frequency (positions squeezed); `factors` [R / 2] divides each by its own,
+    with the rotated dims enlarged by sqrt(1 + ln(length / original_length) /
+    ln(original_length)) once length exceeds original_length."""
+    if R < 2 or R % 2:
+        raise ValueError("R must be even and positive")
+    f = float(base) ** (-np.arange(0, R, 2, dtype=np.float64) / R) / linear
+    factor = 1.0
+    if factors is not None:
+        by = np.asarray(factors, np.float64)
+        if by.shape != f.shape:
+            raise ValueError(f"expected {R // 2} factors, got {list(by.shape)}")
+        f = f / by
+        if length > original_length > 1:
+            factor = float(np.sqrt(1.0 + np.log(length / original_length) / np.log(original_length)))
+    return f.astype(np.float32), factor
+
+
+def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale: float | None = None, window: int = 0,
+                    workspace=None, stream=None):
+    """Causal attention of each sequence's new tokens over its pages: q, out
+    [N, Hq, D] with sequence b's rows cu_q[b] .. cu_q[b + 1], caches
+    [pages, page_size, Hk, D], block_table [B, max_pages], cu_q [B + 1] and
+    kv_len [B] int32 (keys cached, the new tokens' included).  scale: 1 /
+    sqrt(D) if None; window > 0: a token sees the last `window` keys.
+    `workspace`: a uint8 tensor of vxb_paged_attention_workspace bytes, else
+    one is taken from torch's allocator on the call's stream."""
+    import torch
+
+    _rows(q, "q", None, None, None)
+    N, Hq, D = q.shape
+    _rows(k_cache, "k_cache", None, None, None, D)
+    Hk = k_cache.shape[2]
+    pages, page_size, *strides = _cache(k_cache, v_cache, Hk, D, q.dtype)
+    _rows(block_table, "block_table", None, None)
+    B, max_pages = block_table.shape
+    _rows(cu_q, "cu_q", B + 1)
+    _rows(kv_len, "kv_len", B)
+    for t, what in ((block_table, "block_table"), (cu_q, "cu_q"), (kv_len, "kv_len")):
+        _need(t.dtype == torch.int32, f"{what} must be int32")
+    heads, oheads = _heads(q, "q", N, Hq, D, q.dtype), _heads(out, "out", N, Hq, D, q.dtype)
+    if scale is None:
+        scale = D ** -0.5
+    if not q.is_cuda:
+        raise VxbError(ERR_INVALID_ARGUMENT, "paged_attention: tensors must be on one CUDA device")
+    with torch.cuda.device(q.device):
+        need = lib().vxb_paged_attention_workspace(N, B, Hq, Hk, D, max_pages, page_size)
+        if need < 0:
+            raise VxbError(ERR_INVALID_ARGUMENT, lib().vxb_last_error().decode())
+        if workspace is None and need:
+            if stream is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            else:  # memory of the stream that uses it
+                s = torch.cuda.ExternalStream(stream, device=q.device) if isinstance(stream, int) else stream
+                with torch.cuda.stream(s):
+                    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        given = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        _call("paged_attention", (_type_of(q), N, B, Hq, Hk, D, *heads, ptr(k_cache), ptr(v_cache), pages, page_size,
+                                  *strides, ptr(block_table), block_table.stride(0), max_pages, ptr(cu_q),
+                                  ptr(kv_len), scale, window, *oheads, ptr(workspace), given),
+              (q, k_cache, v_cache, block_table, cu_q, kv_len, out, workspace), stream)
