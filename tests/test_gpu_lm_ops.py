@@ -410,7 +410,8 @@ def test_attention_single_tokens(vxb, case, dtype):
 CHUNKS = [  # q_len, kv_len, Hq, Hk, D, page
     ([2], [2], 4, 4, 64, 16), ([37, 5, 1], [1000, 5, 300], 16, 2, 64, 16), ([130], [130], 8, 2, 128, 64),
     ([300, 0, 7, 129], [700, 33, 7, 129], 7, 1, 128, 32), ([65], [4100], 14, 2, 80, 16), ([513], [600], 4, 2, 96, 128),
-    ([16, 3], [16, 2000], 40, 1, 128, 16), ([3, 4], [2, 1], 4, 2, 64, 16), ([256], [1024], 2, 2, 40, 64)]
+    ([16, 3], [16, 2000], 40, 1, 128, 16), ([260], [1500], 2, 1, 128, 256), ([50, 90], [50, 900], 200, 1, 64, 32),
+    ([200, 1, 0, 64], [2000, 900, 7, 6000], 12, 4, 128, 64), ([3, 4], [2, 1], 4, 2, 64, 16), ([256], [1024], 2, 2, 40, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -434,9 +435,10 @@ def test_attention_heads_first_cache_wide_table_and_strided_rows(vxb):
     assert (wide_out[:, 0] == 5).all() and (wide_out[..., 64:] == 5).all()
 
 
-def test_attention_scale_and_zero_scale(vxb):
+@pytest.mark.parametrize("q_len", [5, 150])
+def test_attention_scale_and_zero_scale(vxb, q_len):
     for scale in (0.0, 1.0, -0.3):
-        b = Batch([5, 1], [90, 33], 4, 2, 64, 16, torch.float16)
+        b = Batch([q_len, 1], [q_len + 85, 33], 4, 2, 64, 16, torch.float16)
         b.run(vxb, scale=scale)
         b.check(scale=scale)
 
@@ -479,6 +481,18 @@ def test_attention_non_finite_keys_reach_only_tokens_that_see_them(vxb):
     want = torch.zeros(30, 4, dtype=torch.bool, device="cuda")
     want[20:, :2] = True
     assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_attention_without_pages_or_keys(vxb, q_len):
+    """A cache of no pages, tables of no entries: every token sees nothing and gets zeros."""
+    q = randn(1, q_len, 8, 64, dtype=torch.bfloat16)
+    c = torch.empty(0, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for table in (i(0, 1).view(1, 2), torch.empty(1, 0, dtype=torch.int32, device="cuda")):
+        out = torch.full_like(q, 5.0)
+        vxb.paged_attention(q, c, c, table, i(0, q_len), i(30), out)
+        assert not out.any()
 
 
 def test_attention_lengths_out_of_range_are_cut(vxb):

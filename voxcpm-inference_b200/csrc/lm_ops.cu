@@ -8,7 +8,9 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
+#include "chunk_attn.cuh"
 #include "fp8_gemm.cuh"
 #include "host.h"
 #include "lm_norm.cuh"
@@ -303,40 +305,94 @@ namespace {
 
 constexpr int kAttnMaxD = 128;
 
-// How many parts a call's keys are split into: as many as fill the device
-// with two blocks per SM, no part shorter than 256 keys of a full table.
-int attn_splits(int64_t blocks, int64_t max_keys, int sms) {
-    const int64_t want = 2 * int64_t(sms) / std::max<int64_t>(1, blocks);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_keys / 256, 64})));
+// Which kernel a call takes and into how many parts its keys are split; a
+// function of the extents alone, so that the workspace is known beforehand.
+struct AttnPlan {
+    bool chunk;    // tensor-core kernel for chunks
+    int rows;      // else: rows of a tile
+    int64_t slots; // tile slots over the tokens
+    int groups;    // tiles that a group of heads takes
+    int splits;
+};
+
+AttnPlan attn_plan(int64_t N, int B, int Hq, int Hk, int max_pages, int page_size, int sms,
+                   bool chunks = true) {
+    const int G = Hq / Hk;
+    const int64_t keys = int64_t(max_pages) * page_size;
+    AttnPlan p{};
+    p.chunk = chunks && N * G > int64_t(B) * 64;
+    p.rows = p.chunk ? 128 : N * G > int64_t(B) * 16 ? 32 : 16;
+    const int TT = std::max(1, p.rows / G) * (p.chunk ? 2 : 1), GT = std::min(G, p.rows);
+    p.slots = N / TT + B;
+    p.groups = (G + GT - 1) / GT;
+    // as many parts as fill the device (two blocks per SM, one of the chunk kernel), each of 256
+    // keys (512) at least
+    const int64_t blocks = std::max<int64_t>(1, p.slots * Hk * p.groups);
+    const int64_t want = (p.chunk ? sms : 2 * int64_t(sms)) / blocks;
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / (p.chunk ? 512 : 256), 64})));
+    return p;
 }
 
-int64_t attn_blocks(int64_t N, int B, int Hk, int G, int rows) {
-    const int TT = std::max(1, rows / G), GT = std::min(G, rows);
-    return (N / TT + B) * Hk * ((G + GT - 1) / GT);
-}
-
-int attn_rows(int64_t N, int B, int G) { return N * G > int64_t(B) * 16 ? 32 : 16; }
-
-template <typename T, int DP, int MT>
-int launch_attn(const AttnArgs& a, int dev, cudaStream_t st) {
-    using Cfg = AttnCfg<T, DP, MT>;
-    static std::atomic<bool> attr[64];
-    int rc = allow_smem(attn_rows_kernel<T, DP, MT>, Cfg::kSmemBytes, attr, dev);
-    if (rc) return rc;
-    const int TT = std::max(1, Cfg::kRows / a.G), GT = std::min(a.G, Cfg::kRows);
-    const dim3 g(static_cast<unsigned>(a.N / TT + a.B), static_cast<unsigned>(a.Hk * ((a.G + GT - 1) / GT)),
-                 static_cast<unsigned>(a.splits));
-    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, a));
-    if (a.splits > 1)
-        CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>((a.N * a.Hq + 3) / 4)), dim3(128), 0, st,
-                            a));
+int make_tmap_16(CUtensorMap* m, bool bf16, const void* base, int rank, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled unavailable");
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                     const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled (16 bit) failed: " + std::to_string(r));
     return VXB_OK;
 }
 
 template <typename T>
-int launch_attn_t(const AttnArgs& a, int rows, int dev, cudaStream_t st) {
-    if (a.D <= 64) return rows == 16 ? launch_attn<T, 64, 1>(a, dev, st) : launch_attn<T, 64, 2>(a, dev, st);
-    return rows == 16 ? launch_attn<T, 128, 1>(a, dev, st) : launch_attn<T, 128, 2>(a, dev, st);
+int launch_join(const AttnArgs& a, cudaStream_t st) {
+    CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>((a.N * a.Hq + 3) / 4)), dim3(128), 0, st, a));
+    return VXB_OK;
+}
+
+template <typename T, int DP>
+int launch_chunk(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+    using Cfg = ChunkCfg<DP>;
+    constexpr bool bf = !std::is_same<T, __half>::value;
+    static std::atomic<bool> attr[64];
+    int rc = allow_smem(attn_chunk_kernel<T, DP>, Cfg::kSmemBytes, attr, dev);
+    if (rc) return rc;
+    const cuuint32_t GT = std::min(a.G, 128);
+    const cuuint64_t D = a.D;
+    const auto pitch = [](int64_t elements) { return static_cast<cuuint64_t>(elements) * 2; };
+    CUtensorMap tq, tk, tv;
+    const cuuint64_t qd[3] = {D, static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.N)};
+    const cuuint64_t qs[2] = {pitch(a.q_head), pitch(a.q_token)};
+    const cuuint32_t qb[3] = {64, GT, 128 / GT};
+    if ((rc = make_tmap_16(&tq, bf, a.q, 3, qd, qs, qb))) return rc;
+    const cuuint64_t kd[4] = {D, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.Hk),
+                              static_cast<cuuint64_t>(a.pages)};
+    const cuuint64_t ks[3] = {pitch(a.slot_stride), pitch(a.cache_head), pitch(a.page_stride)};
+    const cuuint32_t kb[4] = {64, static_cast<cuuint32_t>(std::min(a.page_size, kCkStep)), 1, 1};
+    if ((rc = make_tmap_16(&tk, bf, a.k, 4, kd, ks, kb))) return rc;
+    if ((rc = make_tmap_16(&tv, bf, a.v, 4, kd, ks, kb))) return rc;
+    const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
+    CUDA_TRY(launch_pdl(attn_chunk_kernel<T, DP>, g, dim3(kCkThreads), Cfg::kSmemBytes, st, tq, tk, tv, a));
+    return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
+}
+
+template <typename T, int DP, int MT>
+int launch_rows(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+    using Cfg = AttnCfg<T, DP, MT>;
+    static std::atomic<bool> attr[64];
+    int rc = allow_smem(attn_rows_kernel<T, DP, MT>, Cfg::kSmemBytes, attr, dev);
+    if (rc) return rc;
+    const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
+    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, a));
+    return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
+}
+
+template <typename T>
+int launch_attn(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+    if (p.chunk) return a.D <= 64 ? launch_chunk<T, 64>(a, p, dev, st) : launch_chunk<T, 128>(a, p, dev, st);
+    if (a.D <= 64) return p.rows == 16 ? launch_rows<T, 64, 1>(a, p, dev, st) : launch_rows<T, 64, 2>(a, p, dev, st);
+    return p.rows == 16 ? launch_rows<T, 128, 1>(a, p, dev, st) : launch_rows<T, 128, 2>(a, p, dev, st);
 }
 
 int check_attn(const char* op, int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size) {
@@ -359,8 +415,7 @@ extern "C" int64_t vxb_paged_attention_workspace(int64_t N, int B, int Hq, int H
                : [&]() -> int64_t {
         int dev = 0;
         if (cudaGetDevice(&dev) != cudaSuccess) return -1;
-        const int G = Hq / Hk, rows = attn_rows(N, B, G);
-        const int splits = attn_splits(attn_blocks(N, B, Hk, G, rows), int64_t(max_pages) * page_size, num_sms(dev));
+        const int splits = attn_plan(N, B, Hq, Hk, max_pages, page_size, num_sms(dev)).splits;
         return splits > 1 ? int64_t(splits) * N * Hq * (D + 1) * 4 : 0;
     }();
 }
@@ -377,7 +432,7 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         int rc = check_attn(op, N, B, Hq, Hk, D, max_pages, page_size);
         if (rc) return rc;
         if (type != VXB_TYPE_F16 && type != VXB_TYPE_BF16) return bad(op, "the type must be f16 or bf16");
-        if (pages < 0) return bad(op, "bad page count");
+        if (pages < 0 || pages >= (int64_t(1) << 31)) return bad(op, "bad page count");
         if (window < 0) return bad(op, "the window must not be negative");
         if (std::isnan(scale) || std::isinf(scale)) return bad(op, "the scale must be finite");
         if (N == 0 || B == 0) return VXB_OK;
@@ -388,6 +443,10 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || q_token % 8 || q_head % 8 ||
             page_stride % 8 || slot_stride % 8 || head_stride % 8)
             return bad(op, "queries and cache need 16-byte aligned bases and strides");
+        constexpr int64_t far = int64_t(1) << 38;  // a tensor map's strides are below 2^40 bytes
+        if (q_token < 0 || q_head < 0 || page_stride < 0 || slot_stride < 0 || head_stride < 0 || q_token > far ||
+            q_head > far || page_stride > far || slot_stride > far || head_stride > far)
+            return bad(op, "strides of queries and cache must not be negative or beyond 2^38");
         if (!aligned(out, 2) || !aligned(block_table, 4) || !aligned(cu_q, 4) || !aligned(kv_len, 4))
             return bad(op, "a pointer is not aligned to its element");
         int dev = 0;
@@ -401,9 +460,13 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         a.N = N, a.pages = k_cache ? pages : 0, a.B = B, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk, a.D = D;
         a.page_size = page_size, a.max_pages = max_pages, a.window = window;
         while ((1 << a.page_shift) < page_size) ++a.page_shift;
-        a.scale_log2 = scale * 1.4426950408889634f;
-        const int rows = attn_rows(N, B, a.G);
-        a.splits = attn_splits(attn_blocks(N, B, Hk, a.G, rows), int64_t(max_pages) * page_size, num_sms(dev));
+        // (a scale of 0 weighs every key alike; the smallest normal number does too, and keeps
+        // a masked score, -inf, times it -inf)
+        a.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale * 1.4426950408889634f;
+        AttnPlan p = attn_plan(N, B, Hq, Hk, max_pages, page_size, num_sms(dev));
+        // a cache without pages: no key is seen, and a tensor map has no empty axis
+        if (a.pages == 0) p = attn_plan(N, B, Hq, Hk, 0, page_size, num_sms(dev), false);
+        a.splits = p.splits;
         if (a.splits > 1) {
             const int64_t need = int64_t(a.splits) * N * Hq * (D + 1) * 4;
             if (!workspace || workspace_bytes < need || !aligned(workspace, 4))
@@ -412,7 +475,7 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
             a.part_lse = a.part_o + int64_t(a.splits) * N * Hq * D;
         }
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return type == VXB_TYPE_F16 ? launch_attn_t<__half>(a, rows, dev, st)
-                                    : launch_attn_t<__nv_bfloat16>(a, rows, dev, st);
+        return type == VXB_TYPE_F16 ? launch_attn<__half>(a, p, dev, st)
+                                    : launch_attn<__nv_bfloat16>(a, p, dev, st);
     });
 }
