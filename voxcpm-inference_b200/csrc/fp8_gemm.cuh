@@ -104,7 +104,10 @@ struct Fp8Cfg {
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kBufCols = BN < 32 ? 32 : BN;
     static constexpr int kTmemCols = 2 * kBufCols;
-    static constexpr int kRedBytes = BN * 128 * 4;      // split: partial sums [BN][128], over the stages
+    // split: partial sums over the stages, [BN][128] (weights as rows) or [128][BN + 1] (tokens
+    // as rows), so that lanes along the output's fast axis read neighbouring words
+    static constexpr int kRedBytes = 128 * (BN + 1) * 4;
+    static __device__ __forceinline__ int red_at(int row, int col) { return WROWS ? col * 128 + row : row * (BN + 1) + col; }
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
     static_assert(kRedBytes <= kStages * kStageBytes, "partial sums fit the drained stages");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
@@ -119,6 +122,33 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type)
         static_cast<__half*>(y)[i] = __float2half_rn(v);
     } else {
         static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+    }
+}
+
+// n consecutive outputs of a row from column c (8 at a time, n a multiple of
+// 8): vectors where the address and the row's end allow it.
+template <typename T, int NV>
+__device__ __forceinline__ void store_cols(T* y, int c, int M, const float* bias, const float* acc) {
+    constexpr int kVec = 32 / sizeof(T);  // elements of a 32-byte store (a whole sector of the row)
+    const bool fast = (reinterpret_cast<uintptr_t>(y + c) & 31) == 0;
+#pragma unroll
+    for (int i = 0; i < NV; i += kVec) {
+        float v[kVec];
+#pragma unroll
+        for (int x = 0; x < kVec; ++x) v[x] = acc[i + x] + (bias && c + i + x < M ? __ldg(bias + c + i + x) : 0.f);
+        if (fast && c + i + kVec <= M) {
+            uint32_t w[8];
+            T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (int x = 0; x < kVec; ++x) e[x] = from_float<T>(v[x]);
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y + c + i), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        } else {
+#pragma unroll
+            for (int x = 0; x < kVec; ++x)
+                if (c + i + x < M) y[c + i + x] = from_float<T>(v[x]);
+        }
     }
 }
 
@@ -296,10 +326,10 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             }
             if (!ok) break;
             if (split > 1) {
-                // partial sums [column][row] over the drained stages (one tile per cluster)
+                // partial sums over the drained stages (one tile per cluster)
                 float* red = reinterpret_cast<float*>(stages);
 #pragma unroll
-                for (int i = 0; i < NC; ++i) red[(eg * NC + i) * 128 + row] = acc[i];
+                for (int i = 0; i < NC; ++i) red[Cfg::red_at(row, eg * NC + i)] = acc[i];
                 break;
             }
             if (WROWS) {
@@ -309,11 +339,14 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                     if (r < args.M && c0 + i < args.N)
                         store_out(args.y, (c0 + i) * args.y_stride + r, acc[i] + b, args.out_type);
             } else if (r < args.N) {
-#pragma unroll
-                for (int i = 0; i < NC; ++i)
-                    if (c0 + i < args.M)
-                        store_out(args.y, r * args.y_stride + c0 + i, acc[i] + (args.bias ? args.bias[c0 + i] : 0.f),
-                                  args.out_type);
+                const int64_t at = r * args.y_stride;
+                if (args.out_type == kOutF32) {
+                    store_cols<float, NC>(static_cast<float*>(args.y) + at, c0, args.M, args.bias, acc);
+                } else if (args.out_type == kOutF16) {
+                    store_cols<__half, NC>(static_cast<__half*>(args.y) + at, c0, args.M, args.bias, acc);
+                } else {
+                    store_cols<__nv_bfloat16, NC>(static_cast<__nv_bfloat16*>(args.y) + at, c0, args.M, args.bias, acc);
+                }
             }
         }
     }
@@ -325,16 +358,14 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             const int r0 = static_cast<int>(tile0 % args.row_tiles) * 128;
             const int64_t c0 = tile0 / args.row_tiles * BN;
             const uint32_t red = smem_u32(stages);
-            // rank's share: columns rank, rank + split, ...; a warp's lanes are neighbours along
-            // the output's fast axis (weights as rows: rows; tokens as rows: columns are the fast
-            // axis of y, rows are read for coalesced shared memory)
+            // rank's share of the tile, a warp's lanes along the output's fast axis
             for (int i = rank * static_cast<int>(blockDim.x) + threadIdx.x; i < BN * 128; i += split * blockDim.x) {
-                const int c = i >> 7, rr = i & 127;
+                const int c = WROWS ? i >> 7 : i % BN, rr = WROWS ? i & 127 : i / BN;
                 const int64_t n = WROWS ? c0 + c : r0 + rr;
                 const int64_t m = WROWS ? r0 + rr : c0 + c;
                 if (n >= args.N || m >= args.M) continue;
                 float v = 0.f;
-                for (int p = 0; p < split; ++p) v += ld_cluster_f32(red + i * 4, p);
+                for (int p = 0; p < split; ++p) v += ld_cluster_f32(red + Cfg::red_at(rr, c) * 4, p);
                 if (args.bias) v += args.bias[m];
                 store_out(args.y, n * args.y_stride + m, v, args.out_type);
             }
