@@ -47,15 +47,6 @@ struct ChunkCfg {
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z,
-                                            int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(smem_u32(smem_dst)),
-        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // D[tmem] (+)= A[tmem] * B[smem]^T, kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -149,9 +140,11 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         *abort_flag = 0;
         *poison = 0;
         fence_barrier_init();
-        prefetch_tmap(&tmap_q);
-        prefetch_tmap(&tmap_k);
-        prefetch_tmap(&tmap_v);
+        if (a.pages > 0) {
+            prefetch_tmap(&tmap_q);
+            prefetch_tmap(&tmap_k);
+            prefetch_tmap(&tmap_v);
+        }
     }
     grid_dep_sync();
     // (the last tokens of a sequence see most keys: their blocks start first)
@@ -297,8 +290,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                             bad = true;
                             e[x] = from_float<T>(0.f);
                         }
-                    if (bad) {
-                        found = true;
+                    if (bad) {  // (what lies behind the last key is nobody's)
+                        found = found || (my_lo + (i >> 1)) * kCkStep + ((c >> 3) & 127) < key_hi;
                         v[c] = raw;
                     }
                 }

@@ -315,12 +315,11 @@ struct AttnPlan {
     int splits;
 };
 
-AttnPlan attn_plan(int64_t N, int B, int Hq, int Hk, int max_pages, int page_size, int sms,
-                   bool chunks = true) {
+AttnPlan attn_plan(int64_t N, int B, int Hq, int Hk, int max_pages, int page_size, int sms) {
     const int G = Hq / Hk;
     const int64_t keys = int64_t(max_pages) * page_size;
     AttnPlan p{};
-    p.chunk = chunks && N * G > int64_t(B) * 64;
+    p.chunk = N * G > int64_t(B) * 64;
     p.rows = p.chunk ? 128 : N * G > int64_t(B) * 16 ? 32 : 16;
     const int TT = std::max(1, p.rows / G) * (p.chunk ? 2 : 1), GT = std::min(G, p.rows);
     p.slots = N / TT + B;
@@ -345,6 +344,16 @@ int make_tmap_16(CUtensorMap* m, bool bf16, const void* base, int rank, const cu
     return VXB_OK;
 }
 
+// A cache [pages][page_size][Hk][D]: boxes of 64 dims and min(page_size, keys) keys of one head.
+int make_tmap_cache(CUtensorMap* m, bool bf16, const void* base, const AttnArgs& a, int keys) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.D), static_cast<cuuint64_t>(a.page_size),
+                                static_cast<cuuint64_t>(a.Hk), static_cast<cuuint64_t>(a.pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.slot_stride) * 2, static_cast<cuuint64_t>(a.cache_head) * 2,
+                                   static_cast<cuuint64_t>(a.page_stride) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(a.page_size, keys)), 1, 1};
+    return make_tmap_16(m, bf16, base, 4, dims, strides, box);
+}
+
 template <typename T>
 int launch_join(const AttnArgs& a, cudaStream_t st) {
     CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>((a.N * a.Hq + 3) / 4)), dim3(128), 0, st, a));
@@ -358,20 +367,17 @@ int launch_chunk(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st)
     static std::atomic<bool> attr[64];
     int rc = allow_smem(attn_chunk_kernel<T, DP>, Cfg::kSmemBytes, attr, dev);
     if (rc) return rc;
-    const cuuint32_t GT = std::min(a.G, 128);
-    const cuuint64_t D = a.D;
-    const auto pitch = [](int64_t elements) { return static_cast<cuuint64_t>(elements) * 2; };
-    CUtensorMap tq, tk, tv;
-    const cuuint64_t qd[3] = {D, static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.N)};
-    const cuuint64_t qs[2] = {pitch(a.q_head), pitch(a.q_token)};
-    const cuuint32_t qb[3] = {64, GT, 128 / GT};
-    if ((rc = make_tmap_16(&tq, bf, a.q, 3, qd, qs, qb))) return rc;
-    const cuuint64_t kd[4] = {D, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.Hk),
-                              static_cast<cuuint64_t>(a.pages)};
-    const cuuint64_t ks[3] = {pitch(a.slot_stride), pitch(a.cache_head), pitch(a.page_stride)};
-    const cuuint32_t kb[4] = {64, static_cast<cuuint32_t>(std::min(a.page_size, kCkStep)), 1, 1};
-    if ((rc = make_tmap_16(&tk, bf, a.k, 4, kd, ks, kb))) return rc;
-    if ((rc = make_tmap_16(&tv, bf, a.v, 4, kd, ks, kb))) return rc;
+    CUtensorMap tq = {}, tk = {}, tv = {};
+    if (a.pages > 0) {
+        const cuuint32_t GT = std::min(a.G, 128);
+        const cuuint64_t qd[3] = {static_cast<cuuint64_t>(a.D), static_cast<cuuint64_t>(a.Hq),
+                                  static_cast<cuuint64_t>(a.N)};
+        const cuuint64_t qs[2] = {static_cast<cuuint64_t>(a.q_head) * 2, static_cast<cuuint64_t>(a.q_token) * 2};
+        const cuuint32_t qb[3] = {64, GT, 128 / GT};
+        if ((rc = make_tmap_16(&tq, bf, a.q, 3, qd, qs, qb))) return rc;
+        if ((rc = make_tmap_cache(&tk, bf, a.k, a, kCkStep)) || (rc = make_tmap_cache(&tv, bf, a.v, a, kCkStep)))
+            return rc;
+    }
     const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
     CUDA_TRY(launch_pdl(attn_chunk_kernel<T, DP>, g, dim3(kCkThreads), Cfg::kSmemBytes, st, tq, tk, tv, a));
     return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
@@ -384,7 +390,12 @@ int launch_rows(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) 
     int rc = allow_smem(attn_rows_kernel<T, DP, MT>, Cfg::kSmemBytes, attr, dev);
     if (rc) return rc;
     const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
-    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, a));
+    constexpr bool bf = !std::is_same<T, __half>::value;
+    CUtensorMap tk = {}, tv = {};
+    if (a.pages > 0 && ((rc = make_tmap_cache(&tk, bf, a.k, a, kAttnStep)) ||
+                        (rc = make_tmap_cache(&tv, bf, a.v, a, kAttnStep))))
+        return rc;
+    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, tk, tv, a));
     return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
 }
 
@@ -454,18 +465,17 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         AttnArgs a{};
         a.q = q, a.q_token = q_token, a.q_head = q_head;
         a.out = out, a.o_token = o_token, a.o_head = o_head;
-        a.k = k_cache ? k_cache : q, a.v = v_cache ? v_cache : q;  // (pages = 0: addresses only, nothing is read)
+        a.k = k_cache, a.v = v_cache;
         a.page_stride = page_stride, a.slot_stride = slot_stride, a.cache_head = head_stride;
         a.table = block_table, a.table_stride = table_stride, a.cu_q = cu_q, a.kv_len = kv_len;
-        a.N = N, a.pages = k_cache ? pages : 0, a.B = B, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk, a.D = D;
-        a.page_size = page_size, a.max_pages = max_pages, a.window = window;
+        a.N = N, a.pages = pages, a.B = B, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk, a.D = D;
+        // (a cache without pages: no key is seen, nothing is loaded)
+        a.page_size = page_size, a.max_pages = pages ? max_pages : 0, a.window = window;
         while ((1 << a.page_shift) < page_size) ++a.page_shift;
         // (a scale of 0 weighs every key alike; the smallest normal number does too, and keeps
         // a masked score, -inf, times it -inf)
         a.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale * 1.4426950408889634f;
-        AttnPlan p = attn_plan(N, B, Hq, Hk, max_pages, page_size, num_sms(dev));
-        // a cache without pages: no key is seen, and a tensor map has no empty axis
-        if (a.pages == 0) p = attn_plan(N, B, Hq, Hk, 0, page_size, num_sms(dev), false);
+        const AttnPlan p = attn_plan(N, B, Hq, Hk, max_pages, page_size, num_sms(dev));
         a.splits = p.splits;
         if (a.splits > 1) {
             const int64_t need = int64_t(a.splits) * N * Hq * (D + 1) * 4;

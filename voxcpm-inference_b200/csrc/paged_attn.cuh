@@ -10,12 +10,13 @@
 // The G = Hq / Hk query heads that share a key head are rows of one tile
 // (row = token * G + head), so a key is read once for all of them: with one
 // new token per sequence the kernel reads K and V once and is HBM bound.  A
-// block has 4 warps and one tile of 16 * MT rows; a step is 64 keys, of which
-// each warp takes 16: it keeps its own running maximum, sum and output
-// (mma.sync m16n8k16, fp32), so no warp waits for another's softmax, and the
-// four are joined once at the end.  The tensor work of a few rows is far
-// below the time of its bytes, so the accumulators stay in registers and the
-// loads are plain 16-byte cp.async through a ring of kStages steps.
+// block has one tile of 16 * MT rows; a step is 64 keys, of which each of 4
+// warps takes 16: it keeps its own running maximum, sum and output (mma.sync
+// m16n8k16, fp32), so no warp waits for another's softmax, and the four are
+// joined once at the end.  The tensor work of a few rows is far below the time
+// of its bytes, so the accumulators stay in registers.  A fifth warp feeds a
+// ring of kStages steps by TMA, one box per page and 64 dims; it reads the
+// table 32 entries ahead, so a step never waits for its page numbers.
 //
 // With few (sequence, head) pairs the keys are split over blockIdx.z; each
 // part leaves its normalised output and log2 of its sum (fp32), and
@@ -26,12 +27,14 @@
 // 2^-9 of each weight in bf16), the sum is taken of the unrounded weights.
 #pragma once
 
+#include <cuda.h>
+
 #include "lm_norm.cuh"
 
 namespace vxb {
 
 constexpr int kAttnStep = 64;      // keys per step
-constexpr int kAttnThreads = 128;
+constexpr int kAttnThreads = 160;  // 4 warps of rows x keys, one that loads
 constexpr float kNegInf = -INFINITY;
 
 struct AttnArgs {
@@ -87,6 +90,15 @@ struct MmaType<__nv_bfloat16> {
     }
 };
 
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
 __device__ __forceinline__ void ldsm_x4(uint32_t* r, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -138,20 +150,21 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int64_t slot, i
 template <typename T, int DP, int MT>
 struct AttnCfg {
     static constexpr int kRows = 16 * MT;
-    static constexpr int kRowBytes = DP * 2;
-    static constexpr int kTileBytes = kAttnStep * kRowBytes;   // K or V of one step
+    static constexpr int kHalves = DP / 64;
+    static constexpr int kTileBytes = kAttnStep * DP * 2;      // K or V of one step: [half][key][64 dims]
     static constexpr int kStages = DP > 64 ? 3 : 4;
-    static constexpr int kQBytes = kRows * kRowBytes;
-    static constexpr int kSmemBytes = kStages * 2 * kTileBytes + kQBytes;
+    static constexpr int kQBytes = kRows * DP * 2;
+    static constexpr int kSmemBytes = kStages * 2 * kTileBytes + kQBytes + 1024 + 128;
     static constexpr int kJoinBytes = 4 * kRows * DP * 4 + 4 * kRows * 8;  // reuses the ring
     static_assert(kJoinBytes <= kStages * 2 * kTileBytes, "the joining fits the ring");
 };
 
-// Byte offset of 16-byte chunk c of row r in a tile of DP-wide 16-bit rows
-// (chunk index XOR row: ldmatrix reads of 8 rows hit all banks).
-template <int DP>
+// Byte offset of 16-byte chunk c of row r in a tile of R rows of 64 * n dims:
+// [c / 8][r][c % 8] with the 128-byte swizzle (chunk index XOR row), as TMA
+// writes it; ldmatrix reads of 8 rows hit all banks.
+template <int R>
 __device__ __forceinline__ uint32_t attn_off(int r, int c) {
-    return static_cast<uint32_t>(r * DP * 2 + ((c ^ (r & 7)) << 4));
+    return static_cast<uint32_t>((c >> 3) * R * 128 + r * 128 + (((c ^ r) & 7) << 4));
 }
 
 // Sum of the non-finite values of v[.., d] over the keys [j0, j1) of sequence
@@ -170,15 +183,23 @@ __device__ float attn_poison(const AttnArgs& a, const int* table, int head, int 
 }
 
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k,
+                                                                 const __grid_constant__ CUtensorMap tmap_v,
+                                                                 const AttnArgs a) {
     using Cfg = AttnCfg<T, DP, MT>;
     using Mma = MmaType<T>;
     constexpr int S = Cfg::kStages;
+    constexpr int H = Cfg::kHalves;
     constexpr int CH = DP / 8;  // 16-byte chunks of a row
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sq = smem + S * 2 * Cfg::kTileBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sq + Cfg::kQBytes);
+    uint64_t* empty = full + S;
     __shared__ AttnTile sh_tile;
     __shared__ int sh_poison;
+    __shared__ int sh_abort;
+    volatile int* abort_flag = &sh_abort;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int TT = Cfg::kRows / a.G > 0 ? Cfg::kRows / a.G : 1;  // tokens per tile
@@ -186,7 +207,19 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
     const int gparts = (a.G + GT - 1) / GT;                      // tiles a group of heads takes
     const int hk = blockIdx.y / gparts;
     const int g0 = (blockIdx.y % gparts) * GT;
-    if (tid == 0) sh_poison = 0;
+    if (tid == 0) {
+        sh_poison = 0;
+        sh_abort = 0;
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 4);
+        }
+        fence_barrier_init();
+        if (a.pages > 0) {
+            prefetch_tmap(&tmap_k);
+            prefetch_tmap(&tmap_v);
+        }
+    }
     grid_dep_sync();
     const AttnTile t = find_tile(a, blockIdx.x, TT, &sh_tile);
     if (t.b < 0) return;
@@ -198,42 +231,62 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
 
     // keys any row sees, and this part's share of them in whole steps
     const int key_hi = min(t.kv_len, pos0 + toks);
-    int key_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+    const int key_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
     const int step_lo = key_lo / kAttnStep;
     const int step_hi = key_hi > key_lo ? (key_hi + kAttnStep - 1) / kAttnStep : step_lo;
     const int64_t steps = step_hi - step_lo;
     const int my_lo = step_lo + static_cast<int>(steps * blockIdx.z / a.splits);
     const int my_hi = step_lo + static_cast<int>(steps * (blockIdx.z + 1) / a.splits);
 
-    // queries: rows of the tile (zeros past the tokens and past D)
-    for (int i = tid; i < Cfg::kRows * CH; i += kAttnThreads) {
-        const int r = i / CH, c = i % CH;
-        const int tk = r / GT, g = r % GT;
-        const bool on = tk < toks && g < heads && c * 8 < a.D;
-        const T* src = static_cast<const T*>(a.q);
-        if (on) src += (static_cast<int64_t>(t.q0) + t.tok0 + tk) * a.q_token + (hk * a.G + g0 + g) * a.q_head + c * 8;
-        cp_async16(sq + attn_off<DP>(r, c), src, on ? 16 : 0);
-    }
-    auto load_step = [&](int step) {
-        uint8_t* dk = smem + ((step - my_lo) % S) * 2 * Cfg::kTileBytes;
-        uint8_t* dv = dk + Cfg::kTileBytes;
-#pragma unroll 4
-        for (int i = tid; i < kAttnStep * CH; i += kAttnThreads) {
-            const int r = i / CH, c = i % CH;
-            const int j = step * kAttnStep + r;
-            const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
-            const bool on = pg >= 0 && pg < a.pages && c * 8 < a.D;
-            const int64_t off = on ? pg * a.page_stride + (j & (a.page_size - 1)) * a.slot_stride +
-                                         hk * a.cache_head + c * 8
-                                   : 0;
-            cp_async16(dk + attn_off<DP>(r, c), static_cast<const T*>(a.k) + off, on ? 16 : 0);
-            cp_async16(dv + attn_off<DP>(r, c), static_cast<const T*>(a.v) + off, on ? 16 : 0);
+    if (warp == 4) {
+        // -------------------------------------------------- TMA producer --
+        const int box = min(a.page_size, kAttnStep), bps = kAttnStep / box;  // keys of a box, boxes of a step
+        const int per = 32 / bps;                                           // steps whose boxes 32 lanes know
+        auto page = [&](int first) {  // of this lane's box, counted from step `first`
+            const int64_t j = static_cast<int64_t>(first) * kAttnStep + lane * box;
+            return j < key_hi && first < my_hi ? table[j >> a.page_shift] : -1;
+        };
+        const int kv = lane & 1, h = (lane >> 1) % H, bx = (lane >> 1) / H;
+        int next = page(my_lo);
+        bool ok = true;
+        for (int first = my_lo; first < my_hi && ok; first += per) {
+            const int cur = next;
+            next = page(first + per);
+            for (int step = first; step < min(first + per, my_hi); ++step) {
+                const int i = step - my_lo, slot = i % S;
+                int pg = __shfl_sync(0xffffffffu, cur, ((step - first) * bps + bx) & 31);
+                ok = mbar_wait(&empty[slot], ((i / S) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], 2 * Cfg::kTileBytes);
+                __syncwarp();
+                if (bx < bps) {
+                    if (pg < 0 || pg >= a.pages) pg = static_cast<int>(a.pages);  // past the cache: zeros
+                    uint8_t* dst = smem + slot * 2 * Cfg::kTileBytes + kv * Cfg::kTileBytes + h * kAttnStep * 128 +
+                                   bx * box * 128;
+                    tma_load_4d(dst, kv ? &tmap_v : &tmap_k, &full[slot], h * 64,
+                                (step * kAttnStep + bx * box) & (a.page_size - 1), hk, pg);
+                }
+            }
         }
-    };
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) {
-        if (my_lo + s < my_hi) load_step(my_lo + s);
-        asm volatile("cp.async.commit_group;" ::: "memory");  // (the queries go with the first group)
+        if (*abort_flag) {  // give copies already in flight time to land
+            const unsigned long long t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) {
+            }
+        }
+    } else {
+        // queries: rows of the tile (zeros past the tokens and past D)
+        for (int i = tid; i < Cfg::kRows * CH; i += 128) {
+            const int r = i / CH, c = i % CH;
+            const int tk = r / GT, g = r % GT;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (tk < toks && g < heads && c * 8 < a.D)
+                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                    (static_cast<int64_t>(t.q0) + t.tok0 + tk) * a.q_token +
+                                                    (hk * a.G + g0 + g) * a.q_head + c * 8);
+            *reinterpret_cast<uint4*>(sq + attn_off<Cfg::kRows>(r, c)) = v;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
     }
 
     float o[MT][DP / 8][4];
@@ -259,30 +312,41 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
     const int pos_min = pos0, pos_max = pos0 + toks - 1;
     bool poison = false;
 
-    for (int step = my_lo; step < my_hi; ++step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-        __syncthreads();  // the step has landed, and every warp is done with the buffer loaded next
-        if (step + S - 1 < my_hi) load_step(step + S - 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-
-        uint8_t* bk = smem + ((step - my_lo) % S) * 2 * Cfg::kTileBytes;
+    // the tile's Q fragments stay in registers where there is room
+    constexpr bool kQRegs = MT == 1;
+    uint32_t qf[kQRegs ? DP / 16 : 1][4];
+    if (kQRegs && warp < 4) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+            ldsm_x4(qf[kQRegs ? k : 0], smem_u32(sq) + attn_off<Cfg::kRows>(lane & 15, 2 * k + (lane >> 4)));
+    }
+    auto is_absent = [&](int step) {  // does this lane's key (of 16) lie in no page?
+        const int j = step * kAttnStep + warp * 16 + (lane & 15);
+        const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
+        return pg < 0 || pg >= a.pages;
+    };
+    bool gone = warp < 4 && my_lo < my_hi && is_absent(my_lo);
+    bool ok = true;
+    for (int step = warp < 4 ? my_lo : my_hi; step < my_hi; ++step) {
+        const int it = step - my_lo, slot = it % S;
+        uint8_t* bk = smem + slot * 2 * Cfg::kTileBytes;
         uint8_t* bv = bk + Cfg::kTileBytes;
         const int j0 = step * kAttnStep + warp * 16;  // this warp's keys
         // does every row see all of the warp's keys?
         bool whole = j0 + 15 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
         uint32_t absent = 0;  // bit i: key j0 + i lies in no page
-        {
-            const int j = j0 + (lane & 15);
-            const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
-            absent = __ballot_sync(0xffffffffu, pg < 0 || pg >= a.pages) & 0xffffu;
-            whole = whole && absent == 0;
-        }
+        absent = __ballot_sync(0xffffffffu, gone) & 0xffffu;
+        whole = whole && absent == 0;
+        gone = step + 1 < my_hi && is_absent(step + 1);  // (of the next step: its entry is here in time)
+        ok = mbar_wait(&full[slot], (it / S) & 1, abort_flag, nullptr, kErrWaitFull);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (!whole) {
             // A key that some row does not see has weight 0 there, but 0 * inf is NaN: non-finite
             // values leave the tile and are added at the end to the rows that see them.
             for (int i = lane; i < 16 * CH; i += 32) {
                 const int r = warp * 16 + i / CH, c = i % CH;
-                uint4* p = reinterpret_cast<uint4*>(bv + attn_off<DP>(r, c));
+                uint4* p = reinterpret_cast<uint4*>(bv + attn_off<kAttnStep>(r, c));
                 uint4 raw = *p;
                 T* e = reinterpret_cast<T*>(&raw);
                 bool bad = false;
@@ -293,10 +357,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
                         e[x] = from_float<T>(0.f);
                     }
                 if (bad) {
-                    poison = true;
+                    poison = poison || step * kAttnStep + r < key_hi;
                     *p = raw;
                 }
             }
+            fence_proxy_async_smem();  // (before the TMA fills the slot again)
             __syncwarp();
         }
 
@@ -312,11 +377,13 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
         for (int k = 0; k < DP / 16; ++k) {
             uint32_t kb[4];
             // matrices: keys 0-7 and 8-15, each k halves 0-7, 8-15
-            ldsm_x4(kb, smem_u32(bk) + attn_off<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+            ldsm_x4(kb, smem_u32(bk) +
+                            attn_off<kAttnStep>(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                uint32_t qa[4];
-                ldsm_x4(qa, smem_u32(sq) + attn_off<DP>(i * 16 + (lane & 15), 2 * k + (lane >> 4)));
+                uint32_t qs[4];
+                if (!kQRegs) ldsm_x4(qs, smem_u32(sq) + attn_off<Cfg::kRows>(i * 16 + (lane & 15), 2 * k + (lane >> 4)));
+                const uint32_t* qa = kQRegs ? qf[kQRegs ? k : 0] : qs;
                 Mma::mma(s[i][0], qa, kb[0], kb[1]);
                 Mma::mma(s[i][1], qa, kb[2], kb[3]);
             }
@@ -372,22 +439,25 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
         for (int d = 0; d < DP / 16; ++d) {
             uint32_t vb[4];
             // matrices: (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (keys 0-7, dims 8-15), (8-15, 8-15)
-            ldsm_x4_t(vb, smem_u32(bv) + attn_off<DP>(warp * 16 + (lane & 15), 2 * d + (lane >> 4)));
+            ldsm_x4_t(vb, smem_u32(bv) + attn_off<kAttnStep>(warp * 16 + (lane & 15), 2 * d + (lane >> 4)));
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 Mma::mma(o[i][2 * d], pa[i], vb[0], vb[1]);
                 Mma::mma(o[i][2 * d + 1], pa[i], vb[2], vb[3]);
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (poison) sh_poison = 1;
-    __syncthreads();
+    __syncthreads();  // every copy has landed and been read: the ring is free
+    if (*abort_flag) return;
 
     // Join the four warps: each leaves its output, maximum and sum.
     float* jo = reinterpret_cast<float*>(smem);                  // [4][rows][DP]
     float* jm = jo + 4 * Cfg::kRows * DP;                        // [4][rows]
     float* jl = jm + 4 * Cfg::kRows;                             // [4][rows]
+    if (warp < 4) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -405,6 +475,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const AttnArgs 
                 *reinterpret_cast<float2*>(&jo[(warp * Cfg::kRows + r) * DP + j * 8 + (lane & 3) * 2]) =
                     make_float2(o[i][j][2 * h], o[i][j][2 * h + 1]);
         }
+    }
     __syncthreads();
     for (int i = tid; i < Cfg::kRows * DP; i += kAttnThreads) {
         const int r = i / DP, d = i % DP;
