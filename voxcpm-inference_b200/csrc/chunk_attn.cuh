@@ -35,7 +35,6 @@ namespace vxb {
 
 constexpr int kCkStep = 128;        // keys per step
 constexpr int kCkThreads = 384;     // two softmax warpgroups; TMA, MMA and two clearing warps
-constexpr float kCkLazy = 8.f;      // log2 growth of the maximum that O is rescaled for
 
 template <int DP>
 struct ChunkCfg {
@@ -77,12 +76,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // kind::f16 instruction descriptor with A and B of one 16-bit type (format 1
 // = bf16, 0 = f16); b_mn: B is MN-major.
@@ -359,7 +352,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             }
             const float top = fmaxf(t0, t1);
             // rescale if some row of the warp has outgrown its m
-            const bool grow = m == kNegInf ? top > kNegInf : (top - m) * scale > kCkLazy;
+            const bool grow = m == kNegInf ? top > kNegInf : (top - m) * scale > kAttnLazy;
             if (__any_sync(0xffffffffu, grow)) {
                 const float mn = grow ? top : m;
                 const float f = m == mn ? 1.f : ex2((m - mn) * scale);  // 0 from an empty start

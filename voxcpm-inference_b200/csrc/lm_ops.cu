@@ -383,27 +383,27 @@ int launch_chunk(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st)
     return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, int KW>
 int launch_rows(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
-    using Cfg = AttnCfg<T, DP, MT>;
+    using Cfg = AttnCfg<T, DP, MT, KW>;
     static std::atomic<bool> attr[64];
-    int rc = allow_smem(attn_rows_kernel<T, DP, MT>, Cfg::kSmemBytes, attr, dev);
+    int rc = allow_smem(attn_rows_kernel<T, DP, MT, KW>, Cfg::kSmemBytes, attr, dev);
     if (rc) return rc;
     const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
     constexpr bool bf = !std::is_same<T, __half>::value;
     CUtensorMap tk = {}, tv = {};
-    if (a.pages > 0 && ((rc = make_tmap_cache(&tk, bf, a.k, a, kAttnStep)) ||
-                        (rc = make_tmap_cache(&tv, bf, a.v, a, kAttnStep))))
+    if (a.pages > 0 && ((rc = make_tmap_cache(&tk, bf, a.k, a, Cfg::kStep)) ||
+                        (rc = make_tmap_cache(&tv, bf, a.v, a, Cfg::kStep))))
         return rc;
-    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, tk, tv, a));
+    CUDA_TRY(launch_pdl(attn_rows_kernel<T, DP, MT, KW>, g, dim3(kAttnThreads), Cfg::kSmemBytes, st, tk, tv, a));
     return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
 }
 
 template <typename T>
 int launch_attn(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
     if (p.chunk) return a.D <= 64 ? launch_chunk<T, 64>(a, p, dev, st) : launch_chunk<T, 128>(a, p, dev, st);
-    if (a.D <= 64) return p.rows == 16 ? launch_rows<T, 64, 1>(a, p, dev, st) : launch_rows<T, 64, 2>(a, p, dev, st);
-    return p.rows == 16 ? launch_rows<T, 128, 1>(a, p, dev, st) : launch_rows<T, 128, 2>(a, p, dev, st);
+    if (a.D <= 64) return p.rows == 16 ? launch_rows<T, 64, 1, 2>(a, p, dev, st) : launch_rows<T, 64, 2, 2>(a, p, dev, st);
+    return p.rows == 16 ? launch_rows<T, 128, 1, 1>(a, p, dev, st) : launch_rows<T, 128, 2, 1>(a, p, dev, st);
 }
 
 int check_attn(const char* op, int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size) {

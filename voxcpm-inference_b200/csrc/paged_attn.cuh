@@ -10,11 +10,11 @@
 // The G = Hq / Hk query heads that share a key head are rows of one tile
 // (row = token * G + head), so a key is read once for all of them: with one
 // new token per sequence the kernel reads K and V once and is HBM bound.  A
-// block has one tile of 16 * MT rows; a step is 64 keys, of which each of 4
-// warps takes 16: it keeps its own running maximum, sum and output (mma.sync
-// m16n8k16, fp32), so no warp waits for another's softmax, and the four are
-// joined once at the end.  The tensor work of a few rows is far below the time
-// of its bytes, so the accumulators stay in registers.  A fifth warp feeds a
+// block has one tile of 16 * MT rows; a step is 64 * KW keys, of which each
+// of 4 warps takes 16 * KW: it keeps its own running maximum, sum and output
+// (mma.sync m16n8k16, fp32), so no warp waits for another's softmax, and the
+// four are joined once at the end.  The tensor work of a few rows is far below
+// the time of its bytes, so the accumulators stay in registers.  A fifth warp feeds a
 // ring of kStages steps by TMA, one box per page and 64 dims; it reads the
 // table 32 entries ahead, so a step never waits for its page numbers.
 //
@@ -24,7 +24,7 @@
 //
 // exp(s * scale - max) is computed as exp2 of s * scale * log2(e) - max.  P is
 // rounded to the cache's type for the second product (at most half a step,
-// 2^-9 of each weight in bf16), the sum is taken of the unrounded weights.
+// 2^-8 of each weight in bf16), the sum is taken of the unrounded weights.
 #pragma once
 
 #include <cuda.h>
@@ -33,7 +33,7 @@
 
 namespace vxb {
 
-constexpr int kAttnStep = 64;      // keys per step
+constexpr float kAttnLazy = 8.f;   // log2 growth of the maximum that the output is rescaled for
 constexpr int kAttnThreads = 160;  // 4 warps of rows x keys, one that loads
 constexpr float kNegInf = -INFINITY;
 
@@ -99,6 +99,12 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, ui
         : "memory");
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ void ldsm_x4(uint32_t* r, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -147,12 +153,13 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int64_t slot, i
     return *sh;
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, int KW>
 struct AttnCfg {
+    static constexpr int kStep = 64 * KW;                      // keys of a step, 16 * KW a warp
     static constexpr int kRows = 16 * MT;
     static constexpr int kHalves = DP / 64;
-    static constexpr int kTileBytes = kAttnStep * DP * 2;      // K or V of one step: [half][key][64 dims]
-    static constexpr int kStages = DP > 64 ? 3 : 4;
+    static constexpr int kTileBytes = kStep * DP * 2;          // K or V of one step: [half][key][64 dims]
+    static constexpr int kStages = (DP > 64 ? 96 : 64) * 1024 / (2 * kTileBytes);
     static constexpr int kQBytes = kRows * DP * 2;
     static constexpr int kSmemBytes = kStages * 2 * kTileBytes + kQBytes + 1024 + 128;
     static constexpr int kJoinBytes = 4 * kRows * DP * 4 + 4 * kRows * 8;  // reuses the ring
@@ -182,11 +189,12 @@ __device__ float attn_poison(const AttnArgs& a, const int* table, int head, int 
     return s;
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, int KW>
 __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k,
                                                                  const __grid_constant__ CUtensorMap tmap_v,
                                                                  const AttnArgs a) {
-    using Cfg = AttnCfg<T, DP, MT>;
+    using Cfg = AttnCfg<T, DP, MT, KW>;
+    constexpr int kStep = Cfg::kStep;
     using Mma = MmaType<T>;
     constexpr int S = Cfg::kStages;
     constexpr int H = Cfg::kHalves;
@@ -232,18 +240,18 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     // keys any row sees, and this part's share of them in whole steps
     const int key_hi = min(t.kv_len, pos0 + toks);
     const int key_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
-    const int step_lo = key_lo / kAttnStep;
-    const int step_hi = key_hi > key_lo ? (key_hi + kAttnStep - 1) / kAttnStep : step_lo;
+    const int step_lo = key_lo / kStep;
+    const int step_hi = key_hi > key_lo ? (key_hi + kStep - 1) / kStep : step_lo;
     const int64_t steps = step_hi - step_lo;
     const int my_lo = step_lo + static_cast<int>(steps * blockIdx.z / a.splits);
     const int my_hi = step_lo + static_cast<int>(steps * (blockIdx.z + 1) / a.splits);
 
     if (warp == 4) {
         // -------------------------------------------------- TMA producer --
-        const int box = min(a.page_size, kAttnStep), bps = kAttnStep / box;  // keys of a box, boxes of a step
+        const int box = min(a.page_size, kStep), bps = kStep / box;  // keys of a box, boxes of a step
         const int per = 32 / bps;                                           // steps whose boxes 32 lanes know
         auto page = [&](int first) {  // of this lane's box, counted from step `first`
-            const int64_t j = static_cast<int64_t>(first) * kAttnStep + lane * box;
+            const int64_t j = static_cast<int64_t>(first) * kStep + lane * box;
             return j < key_hi && first < my_hi ? table[j >> a.page_shift] : -1;
         };
         const int kv = lane & 1, h = (lane >> 1) % H, bx = (lane >> 1) / H;
@@ -262,10 +270,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
                 __syncwarp();
                 if (bx < bps) {
                     if (pg < 0 || pg >= a.pages) pg = static_cast<int>(a.pages);  // past the cache: zeros
-                    uint8_t* dst = smem + slot * 2 * Cfg::kTileBytes + kv * Cfg::kTileBytes + h * kAttnStep * 128 +
+                    uint8_t* dst = smem + slot * 2 * Cfg::kTileBytes + kv * Cfg::kTileBytes + h * kStep * 128 +
                                    bx * box * 128;
                     tma_load_4d(dst, kv ? &tmap_v : &tmap_k, &full[slot], h * 64,
-                                (step * kAttnStep + bx * box) & (a.page_size - 1), hk, pg);
+                                (step * kStep + bx * box) & (a.page_size - 1), hk, pg);
                 }
             }
         }
@@ -309,6 +317,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
             const int r = i * 16 + h * 8 + (lane >> 2);
             pos[i][h] = r / GT < toks && r % GT < heads ? pos0 + r / GT : -1;
         }
+    const int rows = toks * GT;  // of the tile that hold something
     const int pos_min = pos0, pos_max = pos0 + toks - 1;
     bool poison = false;
 
@@ -320,8 +329,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         for (int k = 0; k < DP / 16; ++k)
             ldsm_x4(qf[kQRegs ? k : 0], smem_u32(sq) + attn_off<Cfg::kRows>(lane & 15, 2 * k + (lane >> 4)));
     }
-    auto is_absent = [&](int step) {  // does this lane's key (of 16) lie in no page?
-        const int j = step * kAttnStep + warp * 16 + (lane & 15);
+    auto is_absent = [&](int step) {  // does this lane's key (of the warp's) lie in no page?
+        const int j = step * kStep + warp * 16 * KW + (lane & (16 * KW - 1));
         const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
         return pg < 0 || pg >= a.pages;
     };
@@ -331,11 +340,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         const int it = step - my_lo, slot = it % S;
         uint8_t* bk = smem + slot * 2 * Cfg::kTileBytes;
         uint8_t* bv = bk + Cfg::kTileBytes;
-        const int j0 = step * kAttnStep + warp * 16;  // this warp's keys
+        const int j0 = step * kStep + warp * 16 * KW;  // this warp's keys
         // does every row see all of the warp's keys?
-        bool whole = j0 + 15 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
-        uint32_t absent = 0;  // bit i: key j0 + i lies in no page
-        absent = __ballot_sync(0xffffffffu, gone) & 0xffffu;
+        bool whole = j0 + 16 * KW - 1 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
+        // bit i: key j0 + i lies in no page
+        const uint32_t absent = __ballot_sync(0xffffffffu, gone);  // (16 keys: in both halves)
         whole = whole && absent == 0;
         gone = step + 1 < my_hi && is_absent(step + 1);  // (of the next step: its entry is here in time)
         ok = mbar_wait(&full[slot], (it / S) & 1, abort_flag, nullptr, kErrWaitFull);
@@ -344,9 +353,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         if (!whole) {
             // A key that some row does not see has weight 0 there, but 0 * inf is NaN: non-finite
             // values leave the tile and are added at the end to the rows that see them.
-            for (int i = lane; i < 16 * CH; i += 32) {
-                const int r = warp * 16 + i / CH, c = i % CH;
-                uint4* p = reinterpret_cast<uint4*>(bv + attn_off<kAttnStep>(r, c));
+            for (int i = lane; i < 16 * KW * CH; i += 32) {
+                const int r = warp * 16 * KW + i / CH, c = i % CH;
+                uint4* p = reinterpret_cast<uint4*>(bv + attn_off<kStep>(r, c));
                 uint4 raw = *p;
                 T* e = reinterpret_cast<T*>(&raw);
                 bool bad = false;
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
                         e[x] = from_float<T>(0.f);
                     }
                 if (bad) {
-                    poison = poison || step * kAttnStep + r < key_hi;
+                    poison = poison || step * kStep + r < key_hi;
                     *p = raw;
                 }
             }
@@ -365,37 +374,46 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
             __syncwarp();
         }
 
-        // S = Q K^T of 16 * MT rows x 16 keys
-        float s[MT][2][4];
+        // S = Q K^T of 16 * MT rows x 16 * KW keys
+        float s[MT][2 * KW][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2 * KW; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-            uint32_t kb[4];
-            // matrices: keys 0-7 and 8-15, each k halves 0-7, 8-15
-            ldsm_x4(kb, smem_u32(bk) +
-                            attn_off<kAttnStep>(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+            uint32_t qs[MT][4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                uint32_t qs[4];
-                if (!kQRegs) ldsm_x4(qs, smem_u32(sq) + attn_off<Cfg::kRows>(i * 16 + (lane & 15), 2 * k + (lane >> 4)));
-                const uint32_t* qa = kQRegs ? qf[kQRegs ? k : 0] : qs;
-                Mma::mma(s[i][0], qa, kb[0], kb[1]);
-                Mma::mma(s[i][1], qa, kb[2], kb[3]);
+            for (int i = 0; i < MT; ++i)
+                if (!kQRegs)
+                    ldsm_x4(qs[i], smem_u32(sq) + attn_off<Cfg::kRows>(i * 16 + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                uint32_t kb[4];
+                // matrices: keys 0-7 and 8-15, each k halves 0-7, 8-15
+                ldsm_x4(kb, smem_u32(bk) + attn_off<kStep>((warp * KW + w) * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                                           2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const uint32_t* qa = kQRegs ? qf[kQRegs ? k : 0] : qs[i];
+                    Mma::mma(s[i][2 * w], qa, kb[0], kb[1]);
+                    Mma::mma(s[i][2 * w + 1], qa, kb[2], kb[3]);
+                }
             }
         }
-        uint32_t pa[MT][4];
+        // Scores in log2 units, hidden ones -inf.  m, the maximum that weights are taken
+        // relative to, follows the true one only when that has outgrown it by 2^8.
+        bool grow = false;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                if (h == 1 && rows <= i * 16 + 8) continue;
                 float top = kNegInf;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2 * KW; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float v = s[i][n][2 * h + e] * a.scale_log2;
@@ -409,43 +427,62 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
                         // (a NaN score has to reach the sum: max ignores it)
                         top = fmaxf(top, v);
                     }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float mn = fmaxf(m[i][h], top);
-                const float base = mn == kNegInf ? 0.f : mn;
-                const float corr = exp2f(m[i][h] - base);
-                m[i][h] = mn;
-                float sum = 0.f;
-                float p[2][2];
+                grow = grow || top > m[i][h] + kAttnLazy;
+            }
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        p[n][e] = exp2f(s[i][n][2 * h + e] - base);
-                        sum += p[n][e];
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1 && rows <= i * 16 + 8) continue;
+                    float top = kNegInf;
+#pragma unroll
+                    for (int n = 0; n < 2 * KW; ++n) top = fmaxf(top, fmaxf(s[i][n][2 * h], s[i][n][2 * h + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float old = m[i][h];
+                    if (top > old + kAttnLazy) m[i][h] = top;
+                    const float corr = m[i][h] == old ? 1.f : ex2(old - m[i][h]);
+                    l[i][h] *= corr;
+#pragma unroll
+                    for (int j = 0; j < DP / 8; ++j) {
+                        o[i][j][2 * h] *= corr;
+                        o[i][j][2 * h + 1] *= corr;
                     }
-                l[i][h] = l[i][h] * corr + sum;
-                pa[i][h] = Mma::pack(p[0][0], p[0][1]);
-                pa[i][2 + h] = Mma::pack(p[1][0], p[1][1]);
+                }
+        }
+        uint32_t pa[MT][KW][4];
 #pragma unroll
-                for (int j = 0; j < DP / 8; ++j) {
-                    o[i][j][2 * h] *= corr;
-                    o[i][j][2 * h + 1] *= corr;
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && rows <= i * 16 + 8) {
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) pa[i][w][1] = pa[i][w][3] = 0;
+                    continue;
+                }
+                const float base = m[i][h] == kNegInf ? 0.f : m[i][h];
+#pragma unroll
+                for (int n = 0; n < 2 * KW; ++n) {
+                    const float p0 = ex2(s[i][n][2 * h] - base), p1 = ex2(s[i][n][2 * h + 1] - base);
+                    l[i][h] += p0 + p1;
+                    pa[i][n >> 1][2 * (n & 1) + h] = Mma::pack(p0, p1);
                 }
             }
-        }
         // O += P V
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            uint32_t vb[4];
-            // matrices: (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (keys 0-7, dims 8-15), (8-15, 8-15)
-            ldsm_x4_t(vb, smem_u32(bv) + attn_off<kAttnStep>(warp * 16 + (lane & 15), 2 * d + (lane >> 4)));
+        for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                Mma::mma(o[i][2 * d], pa[i], vb[0], vb[1]);
-                Mma::mma(o[i][2 * d + 1], pa[i], vb[2], vb[3]);
+            for (int w = 0; w < KW; ++w) {
+                uint32_t vb[4];
+                // matrices: (keys 0-7, dims 0-7), (keys 8-15, dims 0-7), (keys 0-7, dims 8-15), (8-15, 8-15)
+                ldsm_x4_t(vb, smem_u32(bv) + attn_off<kStep>((warp * KW + w) * 16 + (lane & 15), 2 * d + (lane >> 4)));
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    Mma::mma(o[i][2 * d], pa[i][w], vb[0], vb[1]);
+                    Mma::mma(o[i][2 * d + 1], pa[i][w], vb[2], vb[3]);
+                }
             }
-        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[slot]);
     }
@@ -496,8 +533,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         float y = sum == 0.f ? 0.f : val / sum;
         if (sh_poison) {
             const int p = pos0 + tk;
-            const int lo = max(my_lo * kAttnStep, a.window > 0 ? max(0, p - a.window + 1) : 0);
-            const int hi = min(my_hi * kAttnStep, min(p + 1, t.kv_len));
+            const int lo = max(my_lo * kStep, a.window > 0 ? max(0, p - a.window + 1) : 0);
+            const int hi = min(my_hi * kStep, min(p + 1, t.kv_len));
             y += attn_poison<T>(a, table, hk, d, lo, hi);
         }
         const int64_t tok = static_cast<int64_t>(t.q0) + t.tok0 + tk;
