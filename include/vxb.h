@@ -385,8 +385,8 @@ VXB_API int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R,
  * ones too, have no effect.  Rows of q and out outside every sequence are not
  * touched.  type F16 or BF16; D % 8 == 0, D <= 128; page_size a power of two
  * >= 16; q and cache bases and strides multiples of 16 bytes.  `workspace`:
- * vxb_paged_attention_workspace bytes of device memory (0: may be NULL), in
- * use until the call's work on `stream` is done.  Scores, softmax and sums
+ * vxb_paged_attention_workspace bytes of device memory, 16-byte aligned (0:
+ * may be NULL), in use until the call's work on `stream` is done.  Scores, softmax and sums
  * are fp32; the weights are rounded to `type` for the second product. */
 VXB_API int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, int D, const void* q, int64_t q_token,
                                 int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages,

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     __shared__ AttnTile sh_tile;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int GT = min(a.G, 128), TT = 128 / GT;
+    const int GT = min(a.G, 128), TT = a.tokens / 2;
     const int gparts = (a.G + GT - 1) / GT;
     const int hk = blockIdx.y / gparts;
     const int g0 = (blockIdx.y % gparts) * GT;

@@ -310,6 +310,7 @@ constexpr int kAttnMaxD = 128;
 struct AttnPlan {
     bool chunk;    // tensor-core kernel for chunks
     int rows;      // else: rows of a tile
+    int tokens;    // tokens of a tile
     int64_t slots; // tile slots over the tokens
     int groups;    // tiles that a group of heads takes
     int splits;
@@ -321,14 +322,17 @@ AttnPlan attn_plan(int64_t N, int B, int Hq, int Hk, int max_pages, int page_siz
     AttnPlan p{};
     p.chunk = N * G > int64_t(B) * 64;
     p.rows = p.chunk ? 128 : N * G > int64_t(B) * 16 ? 32 : 16;
-    const int TT = std::max(1, p.rows / G) * (p.chunk ? 2 : 1), GT = std::min(G, p.rows);
-    p.slots = N / TT + B;
+    const int GT = std::min(G, p.rows);
+    // tokens of a tile; single tokens (no more of them than sequences) get a tile each
+    p.tokens = p.chunk ? 2 * (128 / GT) : N <= B ? 1 : std::max(1, p.rows / G);
+    p.slots = p.tokens == 1 ? N : N / p.tokens + B;
     p.groups = (G + GT - 1) / GT;
     // as many parts as fill the device (two blocks per SM, one of the chunk kernel), each of 256
     // keys (512) at least
     const int64_t blocks = std::max<int64_t>(1, p.slots * Hk * p.groups);
     const int64_t want = (p.chunk ? sms : 2 * int64_t(sms)) / blocks;
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / (p.chunk ? 512 : 256), 64})));
+    if (getenv("VXB_SPL")) { p.splits=atoi(getenv("VXB_SPL")); return p; }
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / (p.chunk ? 512 : 256), kAttnMaxSplits})));
     return p;
 }
 
@@ -356,7 +360,7 @@ int make_tmap_cache(CUtensorMap* m, bool bf16, const void* base, const AttnArgs&
 
 template <typename T>
 int launch_join(const AttnArgs& a, cudaStream_t st) {
-    CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>((a.N * a.Hq + 3) / 4)), dim3(128), 0, st, a));
+    CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(a.N * a.Hq)), dim3(128), 0, st, a));
     return VXB_OK;
 }
 
@@ -477,10 +481,11 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         a.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale * 1.4426950408889634f;
         const AttnPlan p = attn_plan(N, B, Hq, Hk, max_pages, page_size, num_sms(dev));
         a.splits = p.splits;
+        a.tokens = p.tokens;
         if (a.splits > 1) {
             const int64_t need = int64_t(a.splits) * N * Hq * (D + 1) * 4;
-            if (!workspace || workspace_bytes < need || !aligned(workspace, 4))
-                return bad(op, "the workspace is smaller than vxb_paged_attention_workspace says");
+            if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+                return bad(op, "the workspace is smaller than vxb_paged_attention_workspace says, or not 16-byte aligned");
             a.part_o = static_cast<float*>(workspace);
             a.part_lse = a.part_o + int64_t(a.splits) * N * Hq * D;
         }

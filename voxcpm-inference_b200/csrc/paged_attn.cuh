@@ -55,6 +55,7 @@ struct AttnArgs {
     int page_size, page_shift;
     int max_pages;                 // entries of a table row
     int window;
+    int tokens;                    // tokens of a tile
     float scale_log2;              // softmax scale * log2(e)
     int splits;
     float* part_o;                 // [splits][N * Hq][D]
@@ -118,6 +119,10 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t* r, uint32_t addr) {
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p) : "memory");
+}
+
 // A tile of query rows: which sequence, its tokens and keys.
 struct AttnTile {
     int b;            // -1: nothing to do
@@ -129,26 +134,35 @@ struct AttnTile {
 // Tile slots of TT tokens are numbered so that sequence b starts at slot
 // cu_q[b] / TT + b: the next sequence's start is at least ceil(q_len / TT)
 // later, so every tile has a slot and a slot finds its sequence from cu_q
-// alone, with no sum over the sequences before it.  Lengths out of range (the
-// table's capacity, the rows of q) are cut.  All threads call it.
+// alone, with no sum over the sequences before it.  With TT = 1 a slot is a
+// token.  Lengths out of range (the table's capacity, the rows of q) are cut.
+__device__ __forceinline__ bool tile_of(const AttnArgs& a, int b, int64_t slot, int TT, AttnTile* t) {
+    const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+    const int kv = a.kv_len[b];
+    const int64_t t0 = TT == 1 ? slot - lo : (slot - (lo / TT + b)) * TT;
+    if (lo < 0 || hi <= lo || hi > a.N || t0 < 0 || t0 >= hi - lo) return false;
+    const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page_size;
+    t->b = b;
+    t->tok0 = static_cast<int>(t0);
+    t->q0 = lo;
+    t->q_len = hi - lo;
+    t->kv_len = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kv), cap)));
+    return true;
+}
+
+// The tile of a slot; all threads call it.  In a batch of single tokens a slot
+// is its sequence: one round trip to memory, no search.
 __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int64_t slot, int TT, AttnTile* sh) {
+    AttnTile t;
+    t.b = -1;
+    if (TT == 1 && slot < a.B && tile_of(a, static_cast<int>(slot), slot, TT, &t)) {
+        __syncthreads();
+        return t;
+    }
     if (threadIdx.x == 0) sh->b = -1;
     __syncthreads();
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
-        const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
-        const int kv = a.kv_len[b];
-        if (lo < 0 || hi <= lo || hi > a.N) continue;
-        const int64_t base = lo / TT + b;
-        const int64_t t0 = (slot - base) * TT;
-        if (slot >= base && t0 < hi - lo) {
-            const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page_size;
-            sh->b = b;
-            sh->tok0 = static_cast<int>(t0);
-            sh->q0 = lo;
-            sh->q_len = hi - lo;
-            sh->kv_len = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kv), cap)));
-        }
-    }
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x)
+        if (tile_of(a, b, slot, TT, &t)) *sh = t;
     __syncthreads();
     return *sh;
 }
@@ -210,7 +224,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     volatile int* abort_flag = &sh_abort;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int TT = Cfg::kRows / a.G > 0 ? Cfg::kRows / a.G : 1;  // tokens per tile
+    const int TT = a.tokens;                                     // of a tile
     const int GT = min(a.G, Cfg::kRows);                         // heads of the group per tile
     const int gparts = (a.G + GT - 1) / GT;                      // tiles a group of heads takes
     const int hk = blockIdx.y / gparts;
@@ -229,6 +243,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         }
     }
     grid_dep_sync();
+    if (TT == 1 && warp == 4 && blockIdx.x < a.B && lane < a.max_pages)  // most likely the tile's page numbers
+        prefetch_l1(a.table + blockIdx.x * a.table_stride + lane);
     const AttnTile t = find_tile(a, blockIdx.x, TT, &sh_tile);
     if (t.b < 0) return;
     const int toks = min(TT, t.q_len - t.tok0);
@@ -549,40 +565,54 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     }
 }
 
-// out[row] = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max); a warp per row.
+// out[row] = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max), at most
+// kAttnMaxSplits parts: a block per row, lanes hold the parts' weights, a warp
+// adds every fourth part, 4 dims a lane.
+constexpr int kAttnMaxSplits = 64;
+
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+    __shared__ float4 part[4][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dep_sync();
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= a.N * a.Hq) return;
+    const int64_t row = blockIdx.x, rows = a.N * a.Hq;
     const int64_t tok = row / a.Hq;
     const int head = static_cast<int>(row % a.Hq);
     // rows outside every sequence are left as they are
     bool in = false;
-    for (int b = lane; b < a.B; b += 32) {
+    for (int b = threadIdx.x; b < a.B; b += 128) {
         const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
         in = in || (lo >= 0 && hi <= a.N && tok >= lo && tok < hi);
     }
-    if (!__any_sync(0xffffffffu, in)) return;
-    float top = kNegInf;
-    bool nan = false;
-    for (int s = 0; s < a.splits; ++s) {
-        const float v = a.part_lse[s * a.N * a.Hq + row];
-        nan = nan || v != v;
-        top = fmaxf(top, v);
-    }
+    float lse[2], w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) lse[i] = lane + 32 * i < a.splits ? a.part_lse[(lane + 32 * i) * rows + row] : kNegInf;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = fmaxf(lse[0], lse[1]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == kNegInf ? 0.f : top;
-    float sum = 0.f;
-    for (int s = 0; s < a.splits; ++s) sum += exp2f(a.part_lse[s * a.N * a.Hq + row] - base);
-    for (int d = lane; d < a.D; d += 32) {
-        float v = 0.f;
-        for (int s = 0; s < a.splits; ++s) {
-            const float w = exp2f(a.part_lse[s * a.N * a.Hq + row] - base);
-            if (w != 0.f) v += w * a.part_o[(s * a.N * a.Hq + row) * a.D + d];
+    // (a NaN part makes every weight's sum NaN, and with it the row)
+    w[0] = ex2(lse[0] - base);
+    w[1] = ex2(lse[1] - base);
+    float sum = w[0] + w[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int s = warp; s < a.splits; s += 4) {
+        const float f = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+        if (lane * 4 < a.D && f != 0.f) {
+            const float4 o = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.D + lane * 4);
+            v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
         }
-        const float y = sum == 0.f ? 0.f : v / sum;
-        static_cast<T*>(a.out)[tok * a.o_token + head * a.o_head + d] = from_float<T>(nan ? NAN : y);
+    }
+    part[warp][lane] = v;
+    if (!__syncthreads_or(in) || warp > 0 || lane * 4 >= a.D) return;
+    const float* p = reinterpret_cast<const float*>(&part[0][lane]);
+    T* dst = static_cast<T*>(a.out) + tok * a.o_token + head * a.o_head + lane * 4;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const float y = (p[x] + p[128 + x]) + (p[256 + x] + p[384 + x]);
+        dst[x] = from_float<T>(sum == 0.f ? 0.f : y / sum);
     }
 }
 
