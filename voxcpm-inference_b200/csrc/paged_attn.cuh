@@ -176,7 +176,8 @@ struct AttnCfg {
     static constexpr int kStages = (DP > 64 ? 96 : 64) * 1024 / (2 * kTileBytes);
     static constexpr int kQBytes = kRows * DP * 2;
     static constexpr int kSmemBytes = kStages * 2 * kTileBytes + kQBytes + 1024 + 128;
-    static constexpr int kJoinBytes = 4 * kRows * DP * 4 + 4 * kRows * 8;  // reuses the ring
+    static constexpr int kJoinLD = DP + 4;
+    static constexpr int kJoinBytes = 4 * kRows * kJoinLD * 4 + 4 * kRows * 8;  // reuses the ring
     static_assert(kJoinBytes <= kStages * 2 * kTileBytes, "the joining fits the ring");
 };
 
@@ -506,60 +507,77 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     __syncthreads();  // every copy has landed and been read: the ring is free
     if (*abort_flag) return;
 
-    // Join the four warps: each leaves its output, maximum and sum.
-    float* jo = reinterpret_cast<float*>(smem);                  // [4][rows][DP]
-    float* jm = jo + 4 * Cfg::kRows * DP;                        // [4][rows]
-    float* jl = jm + 4 * Cfg::kRows;                             // [4][rows]
+    // Join the four warps: each leaves its output (rows padded by 4 words: no bank
+    // conflicts), maximum and sum; then a thread adds 4 dims of a row.
+    constexpr int LD = Cfg::kJoinLD;
+    float* jo = reinterpret_cast<float*>(smem);                  // [4][rows][LD]
+    float2* jm = reinterpret_cast<float2*>(jo + 4 * Cfg::kRows * LD);  // [rows][4]: maximum, sum
     if (warp < 4) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = i * 16 + h * 8 + (lane >> 2);
-            float sum = l[i][h];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if ((lane & 3) == 0) {
-                jm[warp * Cfg::kRows + r] = m[i][h];
-                jl[warp * Cfg::kRows + r] = sum;
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && rows <= i * 16 + 8) continue;
+                const int r = i * 16 + h * 8 + (lane >> 2);
+                float sum = l[i][h];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if ((lane & 3) == 0) jm[r * 4 + warp] = make_float2(m[i][h], sum);
+#pragma unroll
+                for (int j = 0; j < DP / 8; ++j)
+                    *reinterpret_cast<float2*>(&jo[(warp * Cfg::kRows + r) * LD + j * 8 + (lane & 3) * 2]) =
+                        make_float2(o[i][j][2 * h], o[i][j][2 * h + 1]);
             }
-#pragma unroll
-            for (int j = 0; j < DP / 8; ++j)
-                *reinterpret_cast<float2*>(&jo[(warp * Cfg::kRows + r) * DP + j * 8 + (lane & 3) * 2]) =
-                    make_float2(o[i][j][2 * h], o[i][j][2 * h + 1]);
-        }
     }
     __syncthreads();
-    for (int i = tid; i < Cfg::kRows * DP; i += kAttnThreads) {
-        const int r = i / DP, d = i % DP;
-        const int tk = r / GT, g = r % GT;
-        if (tk >= toks || g >= heads || d >= a.D) continue;
+    const bool poisoned = sh_poison != 0;
+    for (int i = tid; i < rows * (DP / 4); i += kAttnThreads) {
+        const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+        const int tk = TT == 1 ? 0 : r / GT, g = r - tk * GT;
+        if (g >= heads || d >= a.D) continue;
+        float2 ml[4];
         float top = kNegInf;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, jm[w * Cfg::kRows + r]);
+        for (int w = 0; w < 4; ++w) {
+            ml[w] = jm[r * 4 + w];
+            top = fmaxf(top, ml[w].x);
+        }
         const float base = top == kNegInf ? 0.f : top;
-        float sum = 0.f, val = 0.f;
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = exp2f(jm[w * Cfg::kRows + r] - base);
-            sum += f * jl[w * Cfg::kRows + r];
-            val += f * jo[(w * Cfg::kRows + r) * DP + d];
+            const float f = ex2(ml[w].x - base);
+            sum += f * ml[w].y;
+            const float4 x = *reinterpret_cast<const float4*>(&jo[(w * Cfg::kRows + r) * LD + d]);
+            v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
         }
         // (an empty row has sum 0; a NaN score makes the sum NaN)
-        float y = sum == 0.f ? 0.f : val / sum;
-        if (sh_poison) {
+        const float inv = 1.f / sum;
+        float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+        if (sum == 0.f) y[0] = y[1] = y[2] = y[3] = 0.f;
+        if (poisoned) {
             const int p = pos0 + tk;
             const int lo = max(my_lo * kStep, a.window > 0 ? max(0, p - a.window + 1) : 0);
             const int hi = min(my_hi * kStep, min(p + 1, t.kv_len));
-            y += attn_poison<T>(a, table, hk, d, lo, hi);
+            for (int x = 0; x < 4; ++x) y[x] += attn_poison<T>(a, table, hk, d + x, lo, hi);
         }
         const int64_t tok = static_cast<int64_t>(t.q0) + t.tok0 + tk;
         const int head = hk * a.G + g0 + g;
         if (a.splits == 1) {
-            static_cast<T*>(a.out)[tok * a.o_token + head * a.o_head + d] = from_float<T>(y);
+            T* dst = static_cast<T*>(a.out) + tok * a.o_token + head * a.o_head + d;
+            uint2 w;
+            w.x = Mma::pack(y[0], y[1]);
+            w.y = Mma::pack(y[2], y[3]);
+            if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+                *reinterpret_cast<uint2*>(dst) = w;
+            } else {
+                const T* e = reinterpret_cast<const T*>(&w);
+                for (int x = 0; x < 4; ++x) dst[x] = e[x];
+            }
         } else {
             const int64_t row = (blockIdx.z * a.N + tok) * a.Hq + head;
-            a.part_o[row * a.D + d] = y;
+            *reinterpret_cast<float4*>(a.part_o + row * a.D + d) = make_float4(y[0], y[1], y[2], y[3]);
             if (d == 0) a.part_lse[row] = sum == 0.f ? kNegInf : base + log2f(sum);
         }
     }
