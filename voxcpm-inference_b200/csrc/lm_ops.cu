@@ -53,20 +53,27 @@ int guarded(F f) {
 
 // ---------------------------------------------------------------- rms norm --
 
-template <typename T, int NV>
-cudaError_t launch_norm_v(const NormArgs& a, bool vec, int threads, cudaStream_t st) {
+template <typename T, int NV, bool VEC>
+cudaError_t launch_norm_v(const NormArgs& a, int threads, cudaStream_t st) {
     const dim3 g(static_cast<unsigned>(a.N)), b(threads);
-    return vec ? launch_pdl(rms_norm_kernel<T, NV, true>, g, b, 0, st, a)
-               : launch_pdl(rms_norm_kernel<T, NV, false>, g, b, 0, st, a);
+    if (a.scale)
+        return a.res ? launch_pdl(rms_norm_kernel<T, NV, VEC, true, true>, g, b, 0, st, a)
+                     : launch_pdl(rms_norm_kernel<T, NV, VEC, false, true>, g, b, 0, st, a);
+    return a.res ? launch_pdl(rms_norm_kernel<T, NV, VEC, true, false>, g, b, 0, st, a)
+                 : launch_pdl(rms_norm_kernel<T, NV, VEC, false, false>, g, b, 0, st, a);
 }
 
 template <typename T>
 cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     const int vecs = (a.C + 7) / 8;
     const auto threads = [&](int nv) { return std::max(32, (vecs + 32 * nv - 1) / (32 * nv) * 32); };
-    if (threads(1) <= 256) return launch_norm_v<T, 1>(a, vec, threads(1), st);
-    if (threads(2) <= 1024) return launch_norm_v<T, 2>(a, vec, threads(2), st);
-    return launch_norm_v<T, 4>(a, vec, threads(4), st);
+    if (!vec) {  // strides or widths that do not allow 16-byte vectors
+        if (threads(2) <= 1024) return launch_norm_v<T, 2, false>(a, threads(2), st);
+        return launch_norm_v<T, 4, false>(a, threads(4), st);
+    }
+    if (threads(1) <= 256) return launch_norm_v<T, 1, true>(a, threads(1), st);
+    if (threads(2) <= 1024) return launch_norm_v<T, 2, true>(a, threads(2), st);
+    return launch_norm_v<T, 4, true>(a, threads(4), st);
 }
 
 }  // namespace
@@ -96,7 +103,7 @@ extern "C" int vxb_rms_norm(int type, int64_t N, int C, const void* x, int64_t x
             return bad(op, "a pointer is not aligned to its element");
         NormArgs a{x,  residual, sum, w,        y,        y_scale,      N, x_stride, residual_stride, sum_stride,
                    y_stride, scale_stride, C, w_type == VXB_TYPE_F32 && type != VXB_TYPE_F32, eps};
-        const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(y, q8 ? 8 : 16) && aligned(residual, 16) &&
+        const bool vec = C % 8 == 0 && aligned(x, 16) && aligned(w, 16) && aligned(y, q8 ? 8 : 16) && aligned(residual, 16) &&
                          aligned(sum, 16) && x_stride % 8 == 0 && y_stride % 8 == 0 &&
                          (!residual || residual_stride % 8 == 0) && (!sum || sum_stride % 8 == 0);
         cudaStream_t st = static_cast<cudaStream_t>(stream);

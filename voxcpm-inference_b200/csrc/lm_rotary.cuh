@@ -46,6 +46,16 @@ struct RotaryArgs {
     float factor;
 };
 
+// VEC elements moved at once: 16 bytes, or one element.
+template <typename T, int VEC>
+struct VecOf {
+    using type = uint4;
+};
+template <typename T>
+struct VecOf<T, 1> {
+    using type = T;
+};
+
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a) {
     __shared__ float2 cs[kRotTokens][kRotMaxR / 2];
@@ -71,105 +81,86 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     }
     __syncthreads();
 
-    // Items of a token: per rotated head the pair items, then the rest of the
-    // head; then the values.  A half-layout pair item is two vectors of VEC
-    // dims (i.., i + R/2..), an interleaved one a vector of max(VEC, 2) dims.
+    // Items: (token, head, place in the head).  A half-layout pair item is two
+    // vectors of VEC dims (i.. and i + R/2..), an interleaved one a vector of
+    // max(VEC, 2) dims, an item of the rest of a head a vector of VEC; a value
+    // head is walked alike and only copied.  A thread steps through its items
+    // by adding the block's stride in these three digits: no divisions.
     constexpr int kStep = INTER ? (VEC > 1 ? VEC : 2) : VEC;
+    constexpr int kLoads = INTER ? (VEC > 1 ? 1 : 2) : 2;  // vectors of an item
+    constexpr int kAhead = 4;                              // items whose loads are in flight
+    using V = typename VecOf<T, VEC>::type;
     const int pair_items = INTER ? a.R / kStep : half / kStep;
     const int head_items = pair_items + (a.D - a.R) / VEC;
-    const int heads = a.Hq + (a.k.p ? a.Hk : 0);
-    const int v_items = a.v.p ? a.D / VEC : 0;
-    const int rot_items = heads * head_items;
-    const int items = rot_items + a.Hk * v_items;
-    for (int w = threadIdx.x; w < nt * items; w += blockDim.x) {
-        const int t = w / items;
-        int i = w - t * items;
-        const int64_t n = n0 + t;
-        const T* src;
-        T* dst;
-        if (i < rot_items) {
-            int h = i / head_items;
-            i -= h * head_items;
-            if (h < a.Hq) {
-                src = static_cast<const T*>(a.q.p) + n * a.q.token + h * a.q.head;
-                dst = static_cast<T*>(a.q_out.p) + n * a.q_out.token + h * a.q_out.head;
-            } else {
-                h -= a.Hq;
-                src = static_cast<const T*>(a.k.p) + n * a.k.token + h * a.k.head;
-                if (a.slots) {
-                    if (slot_off[t] < 0) continue;
-                    dst = static_cast<T*>(a.k_cache) + slot_off[t] + h * a.cache_head;
+    const int rot_heads = a.Hq + (a.k.p ? a.Hk : 0);
+    const int heads = rot_heads + (a.v.p ? a.Hk : 0);
+    const int stride_i = blockDim.x % head_items, stride_h = blockDim.x / head_items % heads,
+              stride_t = blockDim.x / head_items / heads;
+    int i = threadIdx.x % head_items, h = threadIdx.x / head_items % heads, t = threadIdx.x / head_items / heads;
+    while (t < nt) {
+        V e[kAhead][kLoads];
+        T* dst[kAhead];
+        int at[kAhead];   // place in the head, -1: nothing to do
+        const float2* c[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            at[u] = -1;
+            if (t < nt) {
+                const int64_t n = n0 + t;
+                const T* src;
+                if (h < a.Hq) {
+                    src = static_cast<const T*>(a.q.p) + n * a.q.token + h * a.q.head;
+                    dst[u] = static_cast<T*>(a.q_out.p) + n * a.q_out.token + h * a.q_out.head;
+                    at[u] = i;
                 } else {
-                    dst = static_cast<T*>(a.k_out.p) + n * a.k_out.token + h * a.k_out.head;
-                }
-            }
-            if (i < pair_items) {
-                if (INTER) {
-                    T e[kStep], o[kStep];
-                    const int d = i * kStep;
-                    if (VEC > 1) {
-                        *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(src + d);
+                    const bool key = h < rot_heads;
+                    const int hk = h - (key ? a.Hq : rot_heads);
+                    const HeadsView& in = key ? a.k : a.v;
+                    src = static_cast<const T*>(in.p) + n * in.token + hk * in.head;
+                    if (a.slots) {
+                        dst[u] = static_cast<T*>(key ? a.k_cache : a.v_cache) + slot_off[t] + hk * a.cache_head;
+                        if (slot_off[t] >= 0) at[u] = i;
                     } else {
-#pragma unroll
-                        for (int j = 0; j < kStep; ++j) e[j] = src[d + j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < kStep / 2; ++j) {
-                        const float2 c = cs[t][d / 2 + j];
-                        const float x = to_float(e[2 * j]), y = to_float(e[2 * j + 1]);
-                        o[2 * j] = from_float<T>(x * c.x - y * c.y);
-                        o[2 * j + 1] = from_float<T>(y * c.x + x * c.y);
-                    }
-                    if (VEC > 1) {
-                        *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(o);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kStep; ++j) dst[d + j] = o[j];
-                    }
-                } else {
-                    T e[2][VEC], o[2][VEC];
-                    const int d = i * VEC;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (VEC > 1) {
-                            *reinterpret_cast<uint4*>(e[s]) = *reinterpret_cast<const uint4*>(src + d + s * half);
-                        } else {
-                            e[s][0] = src[d + s * half];
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float2 c = cs[t][d + j];
-                        const float x = to_float(e[0][j]), y = to_float(e[1][j]);
-                        o[0][j] = from_float<T>(x * c.x - y * c.y);
-                        o[1][j] = from_float<T>(y * c.x + x * c.y);
-                    }
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (VEC > 1) {
-                            *reinterpret_cast<uint4*>(dst + d + s * half) = *reinterpret_cast<const uint4*>(o[s]);
-                        } else {
-                            dst[d + s * half] = o[s][0];
-                        }
+                        dst[u] = static_cast<T*>(a.k_out.p) + n * a.k_out.token + hk * a.k_out.head;
+                        at[u] = i;
                     }
                 }
-                continue;
+                // where the item lies, and its angles (null: copied)
+                const bool pair = i < pair_items;
+                const int d = pair ? i * kStep : a.R + (i - pair_items) * VEC;
+                src += d;
+                dst[u] += d;
+                c[u] = pair && h < rot_heads ? &cs[t][INTER ? d / 2 : d] : nullptr;
+                if (at[u] >= 0) {
+                    at[u] = pair ? 1 : 0;
+                    e[u][0] = *reinterpret_cast<const V*>(src);
+                    if (kLoads > 1 && pair) e[u][kLoads - 1] = *reinterpret_cast<const V*>(src + (INTER ? 1 : half));
+                }
             }
-            i = i - pair_items;
-            src += a.R;
-            dst += a.R;
-        } else {
-            i -= rot_items;
-            const int h = i / v_items;
-            i -= h * v_items;
-            if (slot_off[t] < 0) continue;
-            src = static_cast<const T*>(a.v.p) + n * a.v.token + h * a.v.head;
-            dst = static_cast<T*>(a.v_cache) + slot_off[t] + h * a.cache_head;
+            i += stride_i;
+            h += stride_h;
+            t += stride_t;
+            if (i >= head_items) i -= head_items, ++h;
+            if (h >= heads) h -= heads, ++t;
         }
-        if (VEC > 1) {
-            reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-        } else {
-            dst[i] = src[i];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (at[u] < 0) continue;
+            if (c[u]) {
+                T* v = reinterpret_cast<T*>(e[u]);
+                constexpr int kPairs = INTER ? kStep / 2 : VEC;
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    T* x = INTER ? v + 2 * j : v + j;
+                    T* y = INTER ? v + 2 * j + 1 : v + VEC + j;
+                    const float2 r = c[u][j];
+                    const float p = to_float(*x), q = to_float(*y);
+                    *x = from_float<T>(p * r.x - q * r.y);
+                    *y = from_float<T>(q * r.x + p * r.y);
+                }
+            }
+            *reinterpret_cast<V*>(dst[u]) = e[u][0];
+            if (kLoads > 1 && at[u] > 0) *reinterpret_cast<V*>(dst[u] + (INTER ? 1 : half)) = e[u][kLoads - 1];
         }
     }
 }
