@@ -56,17 +56,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -330,7 +319,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             uint32_t sv[128];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32_async(ts + 32 * c, sv + 32 * c);
-            tmem_ld_wait();
+            tmem_ld_wait<128>(sv);
             float* s = reinterpret_cast<float*>(sv);
             if (neg) {
 #pragma unroll
@@ -367,7 +356,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                     for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
                         tmem_ld16_async(to + c, o);
-                        tmem_ld_wait();
+                        tmem_ld_wait<16>(o);
 #pragma unroll
                         for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
                         tmem_st16(to + c, o);
@@ -417,7 +406,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                 uint32_t o[16];
                 if (n > 0) {
                     tmem_ld16_async(to + c, o);
-                    tmem_ld_wait();
+                    tmem_ld_wait<16>(o);
                 }
                 if (on && c < a.D) {
                     float y[16];

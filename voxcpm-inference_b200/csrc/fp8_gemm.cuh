@@ -49,6 +49,7 @@ struct Fp8GemmArgs {
     int64_t y_stride;
     int out_type;
     int split;                 // blocks of a cluster that share a tile's K
+    int tma_out;               // the output's rows allow TMA stores
 };
 
 // Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3 (format 0), dense, both K-major.
@@ -73,7 +74,23 @@ __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// Waits for this thread's TMEM loads; the N registers are not used before it.
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -97,10 +114,14 @@ struct Fp8Cfg {
     static constexpr int kGroups = BN > 64 ? 2 : 1;     // epilogue warpgroups
     static constexpr int kCols = BN / kGroups;          // columns of a warpgroup
     static constexpr int kThreads = 128 + 128 * kGroups;
+    static constexpr bool kLarge = BN == 256;           // tiles fill the SMs
+    static constexpr bool kSplits = !kLarge;
+    static constexpr bool kTmaOut = kLarge;
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = BN * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStagesFit = (224 * 1024 - 2048) / kStageBytes;
+    static constexpr int kOutBytes = kTmaOut ? 4 * kGroups * 4096 : 0;  // output staging, 4 KB a warp
+    static constexpr int kStagesFit = (226 * 1024 - 2048 - kOutBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kBufCols = BN < 32 ? 32 : BN;
     static constexpr int kTmemCols = 2 * kBufCols;
@@ -108,7 +129,7 @@ struct Fp8Cfg {
     // as rows), so that lanes along the output's fast axis read neighbouring words
     static constexpr int kRedBytes = 128 * (BN + 1) * 4;
     static __device__ __forceinline__ int red_at(int row, int col) { return WROWS ? col * 128 + row : row * (BN + 1) + col; }
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + 1024 + 512;
     static_assert(kRedBytes <= kStages * kStageBytes, "partial sums fit the drained stages");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
     static_assert(BN % 16 == 0 && BN <= 256, "UMMA N");
@@ -152,17 +173,49 @@ __device__ __forceinline__ void store_cols(T* y, int c, int M, const float* bias
     }
 }
 
+// The output through shared memory: a warp's 32 rows x NC columns in boxes of
+// 32 rows x 128 bytes (128-byte swizzle), one at a time, by TMA store.
+template <typename T, int NC>
+__device__ __forceinline__ void store_tile(const void* tmap_y, uint8_t* buf, int lane, int row0, int c0,
+                                           const Fp8GemmArgs& args, const float* acc) {
+    constexpr int kCols = 128 / sizeof(T);  // columns of a box
+    constexpr int kE = 16 / sizeof(T);
+#pragma unroll
+    for (int b = 0; b < NC; b += kCols) {
+        if (lane == 0) bulk_wait_read<0>();  // the buffer's last store has read it
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {        // 16-byte chunks of the row
+            uint4 w;
+            T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                const int col = b + c * kE + i;
+                e[i] = from_float<T>(acc[col] + (args.bias && c0 + col < args.M ? __ldg(args.bias + c0 + col) : 0.f));
+            }
+            *reinterpret_cast<uint4*>(buf + lane * 128 + (((c ^ lane) & 7) << 4)) = w;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && row0 < args.N && c0 + b < args.M) {
+            tma_store_2d(tmap_y, buf, c0 + b, row0);
+            bulk_commit();
+        }
+    }
+}
+
 template <int BN, bool WROWS>
 __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                    const Fp8GemmArgs args) {
+                    const __grid_constant__ CUtensorMap tmap_y, const Fp8GemmArgs args) {
     using Cfg = Fp8Cfg<BN, WROWS>;
     constexpr int S = Cfg::kStages;
     constexpr int NC = Cfg::kCols;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(stages + S * Cfg::kStageBytes);
+    uint8_t* out = stages + S * Cfg::kStageBytes;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(out + Cfg::kOutBytes);
     uint64_t* empty_bar = full_bar + S;
     uint64_t* tfull_bar = empty_bar + S;   // product [2] complete
     uint64_t* tempty_bar = tfull_bar + 2;  // product [2] read
@@ -171,7 +224,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int split = args.split;
+    const int split = Cfg::kSplits ? args.split : 1;
     const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
     // this block's share of the k blocks
     const int kb_lo = static_cast<int>(static_cast<int64_t>(args.kb) * rank / split);
@@ -232,8 +285,8 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             for (int64_t tile = tile0; tile < args.tiles && ok; tile += tile_step) {
                 for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
                     const int st = it % S, buf = it & 1;
-                    if (!mbar_wait(&tempty_bar[buf], ((it >> 1) & 1) ^ 1, abort_flag, nullptr, kErrWaitAccum) ||
-                        !mbar_wait(&full_bar[st], (it / S) & 1, abort_flag, nullptr, kErrWaitFull)) {
+                    if (!mbar_wait(&full_bar[st], (it / S) & 1, abort_flag, nullptr, kErrWaitFull) ||
+                        !mbar_wait(&tempty_bar[buf], ((it >> 1) & 1) ^ 1, abort_flag, nullptr, kErrWaitAccum)) {
                         ok = false;
                         break;
                     }
@@ -302,7 +355,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                     uint32_t v[CH];
 #pragma unroll
                     for (int i = 0; i < CH; i += 16) tmem_ld16_async(t + c + i, v + i);
-                    tmem_ld_wait();
+                    tmem_ld_wait<CH>(v);
 #pragma unroll
                     for (int i = 0; i < CH; i += 2) {
                         float2 sc = make_float2(s, s);
@@ -325,7 +378,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                 col2 = col2_n;
             }
             if (!ok) break;
-            if (split > 1) {
+            if (Cfg::kSplits && split > 1) {
                 // partial sums over the drained stages (one tile per cluster)
                 float* red = reinterpret_cast<float*>(stages);
 #pragma unroll
@@ -338,6 +391,16 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                 for (int i = 0; i < NC; ++i)
                     if (r < args.M && c0 + i < args.N)
                         store_out(args.y, (c0 + i) * args.y_stride + r, acc[i] + b, args.out_type);
+            } else if (Cfg::kTmaOut && args.tma_out) {
+                uint8_t* buf = out + (warp - 4) * 4096;
+                const int row0 = r - lane;
+                if (args.out_type == kOutF32) {
+                    store_tile<float, NC>(&tmap_y, buf, lane, row0, c0, args, acc);
+                } else if (args.out_type == kOutF16) {
+                    store_tile<__half, NC>(&tmap_y, buf, lane, row0, c0, args, acc);
+                } else {
+                    store_tile<__nv_bfloat16, NC>(&tmap_y, buf, lane, row0, c0, args, acc);
+                }
             } else if (r < args.N) {
                 const int64_t at = r * args.y_stride;
                 if (args.out_type == kOutF32) {
@@ -351,7 +414,8 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
         }
     }
 
-    if (split > 1) {
+    if (Cfg::kTmaOut && args.tma_out && warp >= 4 && lane == 0) bulk_wait_all();  // stores done before the staging goes
+    if (Cfg::kSplits && split > 1) {
         __syncwarp();
         cluster_arrive_wait();  // every rank's partial sums are written
         if (!*abort_flag && tile0 < args.tiles) {

@@ -242,6 +242,23 @@ int make_tmap_e4m3(CUtensorMap* m, const void* base, uint64_t K, uint64_t rows, 
     return VXB_OK;
 }
 
+// Output [rows][cols] (row pitch in bytes), boxes of 128 bytes x 32 rows.
+int make_tmap_out(CUtensorMap* m, void* base, int type, uint64_t cols, uint64_t rows, uint64_t pitch) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {type == kOutF32 ? 32u : 64u, 32};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(m, type == kOutF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : type == kOutF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                     2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VXB_ERR_BACKEND, "cuTensorMapEncodeTiled (output) failed: " + std::to_string(r));
+    return VXB_OK;
+}
+
 struct Fp8Operands {
     const void *x, *w;
     int64_t x_stride, w_stride;
@@ -259,13 +276,18 @@ int launch_fp8(const Fp8Operands& o, Fp8GemmArgs a, int dev, cudaStream_t st) {
     // fewer tiles than SMs: K is shared by the blocks of a cluster, each with two k blocks at least
     const int sms = num_sms(dev);
     a.split = 1;
-    while (a.split < 8 && a.tiles * a.split * 2 <= sms && a.kb >= a.split * 4) a.split *= 2;
-    CUtensorMap tx, tw;
+    while (Cfg::kSplits && a.split < 8 && a.tiles * a.split * 2 <= sms && a.kb >= a.split * 4) a.split *= 2;
+    CUtensorMap tx, tw, ty = {};
+    if (Cfg::kTmaOut) {
+        const int es = a.out_type == kOutF32 ? 4 : 2;
+        a.tma_out = aligned(a.y, 16) && a.y_stride * es % 16 == 0;
+        if (a.tma_out && (rc = make_tmap_out(&ty, a.y, a.out_type, a.M, a.N, a.y_stride * es))) return rc;
+    }
     if ((rc = make_tmap_e4m3(&tx, o.x, a.K, a.N, o.x_stride, WROWS ? BN : 128))) return rc;
     if ((rc = make_tmap_e4m3(&tw, o.w, a.K, a.M, o.w_stride, WROWS ? 128 : BN))) return rc;
     const int64_t grid = a.split > 1 ? a.tiles * a.split : std::min<int64_t>(a.tiles, sms);
     CUDA_TRY(launch_pdl_cluster(fp8_gemm_kernel<BN, WROWS>, dim3(static_cast<unsigned>(grid)), dim3(Cfg::kThreads),
-                                a.split, Cfg::kSmemBytes, st, WROWS ? tw : tx, WROWS ? tx : tw, a));
+                                a.split, Cfg::kSmemBytes, st, WROWS ? tw : tx, WROWS ? tx : tw, ty, a));
     return VXB_OK;
 }
 
