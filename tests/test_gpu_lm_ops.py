@@ -411,12 +411,13 @@ CHUNKS = [  # q_len, kv_len, Hq, Hk, D, page
     ([2], [2], 4, 4, 64, 16), ([37, 5, 1], [1000, 5, 300], 16, 2, 64, 16), ([130], [130], 8, 2, 128, 64),
     ([300, 0, 7, 129], [700, 33, 7, 129], 7, 1, 128, 32), ([65], [4100], 14, 2, 80, 16), ([513], [600], 4, 2, 96, 128),
     ([16, 3], [16, 2000], 40, 1, 128, 16), ([260], [1500], 2, 1, 128, 256), ([50, 90], [50, 900], 200, 1, 64, 32),
-    ([200, 1, 0, 64], [2000, 900, 7, 6000], 12, 4, 128, 64), ([3, 4], [2, 1], 4, 2, 64, 16), ([256], [1024], 2, 2, 40, 64)]
+    ([200, 1, 0, 64], [2000, 900, 7, 6000], 12, 4, 128, 64),
+    ([9 + b % 3 for b in range(300)], [20 + 7 * b % 90 for b in range(300)], 8, 1, 64, 16), ([3, 4], [2, 1], 4, 2, 64, 16), ([256], [1024], 2, 2, 40, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("window", [0, 1, 50, 100000])
-@pytest.mark.parametrize("case", CHUNKS, ids=str)
+@pytest.mark.parametrize("case", CHUNKS, ids=lambda c: str(c)[:60])
 def test_attention_chunks(vxb, case, window, dtype):
     b = Batch(*case, dtype, window=window, tail=3)
     b.run(vxb)

@@ -46,13 +46,38 @@ struct ChunkCfg {
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, kind::f16.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// One tcgen05.mma, kind::f16, issued by the lane whose `leader` is set of a warp
+// that runs together: in a branch of one lane the operands would have to be
+// carried to uniform registers for every instruction (about 65 clocks each,
+// more than the product of 64 columns takes).  The matrix descriptors are
+// {address >> 4 | leading offset >> 4 << 16, kDescHigh}: 32-bit arithmetic.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride offset 1024, version, 128-byte swizzle
+
+// D[tmem] (+)= A[smem] * B[smem]^T
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t alo, uint32_t blo, uint32_t idesc,
+                                        uint32_t accumulate, uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"
+        " mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(alo), "r"(blo), "r"(kDescHigh), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t blo, uint32_t idesc,
+                                        uint32_t accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"
+        " mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(blo), "r"(kDescHigh), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
         : "memory");
 }
 
@@ -73,6 +98,45 @@ __host__ __device__ constexpr uint32_t make_idesc_16(int M, int N, int b_mn) {
     constexpr uint32_t f = sizeof(T) == 2 && !__is_same(T, __half) ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | (static_cast<uint32_t>(b_mn) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// The tile of a slot when sequences are taken in the order of their keys, the
+// longest first, and a sequence's tiles from its last tokens on: every thread
+// ranks one sequence (B <= kCkSort of them) against all others.  `work`: B
+// entries of shared memory.  All threads call it.
+constexpr int kCkSort = 256;
+
+__device__ __forceinline__ AttnTile find_long_tile(const AttnArgs& a, int64_t slot, int TT, AttnTile* sh, int2* work) {
+    const int b = threadIdx.x;
+    int2 mine = make_int2(0, 0);  // keys, tiles
+    if (b < a.B) {
+        const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+        if (lo >= 0 && hi > lo && hi <= a.N) mine = make_int2(a.kv_len[b], (hi - lo + TT - 1) / TT);
+        work[b] = mine;
+    }
+    if (b == 0) sh->b = -1;
+    __syncthreads();
+    if (mine.y > 0) {
+        int64_t base = 0;
+        for (int o = 0; o < a.B; ++o) {
+            const int2 w = work[o];
+            if (w.x > mine.x || (w.x == mine.x && o < b)) base += w.y;
+        }
+        const int64_t at = slot - base;
+        if (at >= 0 && at < mine.y) {
+            const int lo = a.cu_q[b];
+            const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page_size;
+            AttnTile t;
+            t.b = b;
+            t.tok0 = static_cast<int>(mine.y - 1 - at) * TT;
+            t.q0 = lo;
+            t.q_len = a.cu_q[b + 1] - lo;
+            t.kv_len = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(mine.x), cap)));
+            *sh = t;
+        }
+    }
+    __syncthreads();
+    return *sh;
 }
 
 template <typename T, int DP>
@@ -103,8 +167,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int GT = min(a.G, 128), TT = a.tokens / 2;
     const int gparts = (a.G + GT - 1) / GT;
-    const int hk = blockIdx.y / gparts;
-    const int g0 = (blockIdx.y % gparts) * GT;
+    // blocks in the order (tiles, the longest first; heads): all heads of a tile run together,
+    // and the short tiles fill the end
+    const int heads_y = a.Hk * gparts;
+    const int64_t slot = blockIdx.x / heads_y;
+    const int hy = blockIdx.x % heads_y;
+    const int hk = hy / gparts;
+    const int g0 = (hy % gparts) * GT;
 
     if (tid == 0) {
         for (int i = 0; i < R; ++i) {
@@ -129,8 +198,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
     }
     grid_dep_sync();
-    // (the last tokens of a sequence see most keys: their blocks start first)
-    const AttnTile t = find_tile(a, static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x, 2 * TT, &sh_tile);
+    const AttnTile t = a.B <= kCkSort ? find_long_tile(a, slot, 2 * TT, &sh_tile, reinterpret_cast<int2*>(ring))
+                                      : find_tile(a, gridDim.x / heads_y - 1 - slot, 2 * TT, &sh_tile);
     if (t.b < 0) return;
     if (warp == 9) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
@@ -198,52 +267,56 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         }
     } else if (warp == 9) {
         // ---------------------------------------------------- MMA issuer --
-        if (lane == 0 && steps > 0) {
+        if (steps > 0) {
             constexpr uint32_t idesc_s = make_idesc_16<T>(128, kCkStep, 0);
             constexpr uint32_t idesc_o = make_idesc_16<T>(128, DP, 1);
+            constexpr uint32_t kLow = (16u >> 4) << 16, kLowV = (16384u >> 4) << 16;  // leading offsets
+            const uint32_t leader = lane == 0;
+            const uint32_t q_addr = smem_u32(sq) >> 4, ring_addr = smem_u32(ring) >> 4;
+            auto wait = [&](uint64_t* bar, int parity, int code) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, nullptr, code)) != 0;
+            };
             auto scores = [&](int i, int slot) {  // S_i = Q_i K^T
-                const uint32_t qa = smem_u32(sq) + i * H * 16384, kb = smem_u32(ring) + slot * Cfg::kTileBytes;
+                const uint32_t qa = kLow | (q_addr + i * (H * 16384 / 16));
+                const uint32_t kb = kLow | (ring_addr + slot * (Cfg::kTileBytes / 16));
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                    umma_f16(tmem + i * 128, make_sdesc(qa + off, 16, 1024), make_sdesc(kb + off, 16, 1024), idesc_s,
-                             kk != 0);
+                    const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
+                    umma_ss(tmem + i * 128, qa + off, kb + off, idesc_s, kk != 0, leader);
                 }
-                umma_commit(&s_full[i]);
+                umma_commit_by(&s_full[i], leader);
             };
-            bool ok = mbar_wait(q_bar, 0, abort_flag, nullptr, kErrWaitFull) &&
-                      mbar_wait(&clear[0], 0, abort_flag, nullptr, kErrWaitFull);
+            bool ok = wait(q_bar, 0, kErrWaitFull) && wait(&clear[0], 0, kErrWaitFull);
             if (ok) {
                 tc_fence_after();
                 for (int i = 0; i < tiles; ++i) scores(i, 0);
-                umma_commit(&empty[0]);
+                umma_commit_by(&empty[0], leader);
             }
             for (int j = 0; j < steps && ok; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2;  // ring items of V_j and K_{j+1}
-                ok = mbar_wait(&clear[iv % R], (iv / R) & 1, abort_flag, nullptr, kErrWaitFull);
-                if (ok && j + 1 < steps)
-                    ok = mbar_wait(&clear[ik % R], (ik / R) & 1, abort_flag, nullptr, kErrWaitFull);
+                ok = wait(&clear[iv % R], (iv / R) & 1, kErrWaitFull);
+                if (ok && j + 1 < steps) ok = wait(&clear[ik % R], (ik / R) & 1, kErrWaitFull);
+                const uint32_t vb = kLowV | (ring_addr + (iv % R) * (Cfg::kTileBytes / 16));
                 for (int i = 0; i < tiles && ok; ++i) {
-                    ok = mbar_wait(&p_full[i], j & 1, abort_flag, nullptr, kErrWaitAccum);
+                    ok = wait(&p_full[i], j & 1, kErrWaitAccum);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t vb = smem_u32(ring) + (iv % R) * Cfg::kTileBytes;
 #pragma unroll
                     for (int kk = 0; kk < kCkStep / 16; ++kk)  // 16 keys: 8 TMEM columns of P, 2 KB of V rows
-                        umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, make_sdesc(vb + kk * 2048, 16384, 1024),
-                                    idesc_o, (j | kk) != 0);
-                    umma_commit(&o_done[i]);
-                    if (i == tiles - 1) umma_commit(&empty[iv % R]);
+                        umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vb + kk * (2048 / 16), idesc_o,
+                                (j | kk) != 0, leader);
+                    umma_commit_by(&o_done[i], leader);
+                    if (i == tiles - 1) umma_commit_by(&empty[iv % R], leader);
                     // (in order behind the product that reads P, which these scores overwrite)
                     if (j + 1 < steps) {
                         scores(i, ik % R);
-                        if (i == tiles - 1) umma_commit(&empty[ik % R]);
+                        if (i == tiles - 1) umma_commit_by(&empty[ik % R], leader);
                     }
                 }
             }
             if (!ok) {  // arrives once every issued MMA is done
-                umma_commit(&o_done[0]);
-                umma_commit(&o_done[1]);
+                umma_commit_by(&o_done[0], leader);
+                umma_commit_by(&o_done[1], leader);
             }
         }
         __syncwarp();

@@ -360,7 +360,6 @@ AttnPlan attn_plan(int64_t N, int B, int Hq, int Hk, int max_pages, int page_siz
     // keys (512) at least
     const int64_t blocks = std::max<int64_t>(1, p.slots * Hk * p.groups);
     const int64_t want = (p.chunk ? sms : 2 * int64_t(sms)) / blocks;
-    if (getenv("VXB_SPL")) { p.splits=atoi(getenv("VXB_SPL")); return p; }
     p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / (p.chunk ? 512 : 256), kAttnMaxSplits})));
     return p;
 }
@@ -411,7 +410,7 @@ int launch_chunk(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st)
         if ((rc = make_tmap_cache(&tk, bf, a.k, a, kCkStep)) || (rc = make_tmap_cache(&tv, bf, a.v, a, kCkStep)))
             return rc;
     }
-    const dim3 g(static_cast<unsigned>(p.slots), static_cast<unsigned>(a.Hk * p.groups), static_cast<unsigned>(p.splits));
+    const dim3 g(static_cast<unsigned>(p.slots * a.Hk * p.groups), 1, static_cast<unsigned>(p.splits));
     CUDA_TRY(launch_pdl(attn_chunk_kernel<T, DP>, g, dim3(kCkThreads), Cfg::kSmemBytes, st, tq, tk, tv, a));
     return a.splits > 1 ? launch_join<T>(a, st) : VXB_OK;
 }
@@ -518,6 +517,7 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
             a.part_o = static_cast<float*>(workspace);
             a.part_lse = a.part_o + int64_t(a.splits) * N * Hq * D;
         }
+        if (p.slots * Hk * p.groups >= (int64_t(1) << 31)) return bad(op, "too many tokens for one call");
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         return type == VXB_TYPE_F16 ? launch_attn<__half>(a, p, dev, st)
                                     : launch_attn<__nv_bfloat16>(a, p, dev, st);
