@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                         // (D is a multiple of 8: whole vectors, 32-byte rows)
 #pragma unroll
                         for (int x = 0; x < 16; x += 8)
-                            if (c + x < a.D) store8<float, false>(a.part_o + row * a.D + c + x, 8, y + x);
+                            if (c + x < a.D) store8<float, true>(a.part_o + row * a.D + c + x, 8, y + x);
                     } else if (c + 16 <= a.D && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
                         store8<T, true>(dst, 8, y);
                         store8<T, true>(dst + 8, 8, y + 8);

@@ -388,7 +388,13 @@ int make_tmap_cache(CUtensorMap* m, bool bf16, const void* base, const AttnArgs&
 
 template <typename T>
 int launch_join(const AttnArgs& a, cudaStream_t st) {
-    CUDA_TRY(launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(a.N * a.Hq)), dim3(128), 0, st, a));
+    // a block per row, or a warp where there are rows enough for the device
+    const int64_t rows = a.N * a.Hq;
+    if (rows < 2048) {
+        CUDA_TRY(launch_pdl(attn_join_kernel<T, 4>, dim3(static_cast<unsigned>(rows)), dim3(128), 0, st, a));
+    } else {
+        CUDA_TRY(launch_pdl(attn_join_kernel<T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, a));
+    }
     return VXB_OK;
 }
 

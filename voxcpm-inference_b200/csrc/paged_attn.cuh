@@ -584,21 +584,23 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
 }
 
 // out[row] = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max), at most
-// kAttnMaxSplits parts: a block per row, lanes hold the parts' weights, a warp
-// adds every fourth part, 4 dims a lane.
+// kAttnMaxSplits parts.  `warps` (1 or 4) of a block's 4 warps share a row:
+// lanes hold the parts' weights, a warp adds every `warps`-th part, 4 dims a
+// lane.
 constexpr int kAttnMaxSplits = 64;
 
-template <typename T>
+template <typename T, int kWarps>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     __shared__ float4 part[4][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % kWarps;
     grid_dep_sync();
-    const int64_t row = blockIdx.x, rows = a.N * a.Hq;
+    const int64_t rows = a.N * a.Hq;
+    const int64_t row = min(static_cast<int64_t>(blockIdx.x) * (4 / kWarps) + warp / kWarps, rows - 1);
     const int64_t tok = row / a.Hq;
     const int head = static_cast<int>(row % a.Hq);
     // rows outside every sequence are left as they are
     bool in = false;
-    for (int b = threadIdx.x; b < a.B; b += 128) {
+    for (int b = lane; b < a.B; b += 32) {
         const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
         in = in || (lo >= 0 && hi <= a.N && tok >= lo && tok < hi);
     }
@@ -616,22 +618,32 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     float sum = w[0] + w[1];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    for (int s = warp; s < a.splits; s += 4) {
+#pragma unroll 4
+    for (int s = mine; s < a.splits; s += kWarps) {
         const float f = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
         if (lane * 4 < a.D && f != 0.f) {
             const float4 o = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.D + lane * 4);
             v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
         }
     }
-    part[warp][lane] = v;
-    if (!__syncthreads_or(in) || warp > 0 || lane * 4 >= a.D) return;
-    const float* p = reinterpret_cast<const float*>(&part[0][lane]);
-    T* dst = static_cast<T*>(a.out) + tok * a.o_token + head * a.o_head + lane * 4;
+    in = __any_sync(0xffffffffu, in);
+    if (kWarps > 1) {
+        part[warp][lane] = v;
+        __syncthreads();
+        if (warp > 0) return;
+        v = part[0][lane];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float y = (p[x] + p[128 + x]) + (p[256 + x] + p[384 + x]);
-        dst[x] = from_float<T>(sum == 0.f ? 0.f : y / sum);
+        for (int i = 1; i < kWarps; ++i) {
+            const float4 o = part[i][lane];
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
     }
+    if (!in || lane * 4 >= a.D) return;
+    T* dst = static_cast<T*>(a.out) + tok * a.o_token + head * a.o_head + lane * 4;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) dst[x] = from_float<T>(y[x]);
 }
 
 }  // namespace vxb
