@@ -1,24 +1,28 @@
-"""Builds libvxb.so (CUDA kernels + C ABI + C++ host API) for sm_100a, in-tree.
+"""Builds libvxb.so (CUDA kernels + C ABI + C++ host API) for sm_100a and the
+Python module _vxb_native.so (torch tensors to the C ABI), in-tree.
 
     python voxcpm-inference_b200/build.py [-v]
 
-Objects go to voxcpm-inference_b200/_build/, the library to
-voxcpm-inference_b200/lib/libvxb.so.  Only files whose sources (or shared
+Objects go to voxcpm-inference_b200/_build/, the libraries to
+voxcpm-inference_b200/lib/.  Only files whose sources (or shared
 headers) changed are recompiled.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "lib", "libvxb.so")
+NATIVE = os.path.join(PKG, "lib", "_vxb_native.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 INC = ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-I" + os.path.join(PKG, "include")]
@@ -28,6 +32,10 @@ def _sources():
     cu = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     cpp = sorted(glob.glob(os.path.join(CSRC, "*.cpp")) + glob.glob(os.path.join(CSRC, "host", "*.cpp")))
     return cu, cpp
+
+
+def _torch():
+    return importlib.util.find_spec("torch").submodule_search_locations[0]
 
 
 def _headers():
@@ -69,12 +77,26 @@ def build(verbose: bool = False) -> str:
         if _stale(o, s, hdr_mtime):
             jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
                          "-I/usr/local/cuda/include", *INC, "-c", s, "-o", o])
+    bind, bind_obj = os.path.join(CSRC, "bind", "native.cpp"), os.path.join(BUILD, "native.cpp.o")
+    abi = os.path.join(ROOT, "include", "vxb.h")
+    bind_stale = _stale(bind_obj, bind, max(os.path.getmtime(abi), os.path.getmtime(__file__)))
+    if bind_stale:
+        inc = os.path.join(_torch(), "include")
+        jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-I" + inc,
+                     "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+                     "-I" + sysconfig.get_paths()["include"], "-I/usr/local/cuda/include", *INC, "-c", bind, "-o",
+                     bind_obj])
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
         for out in ex.map(lambda c: _run(c, verbose), jobs):
             if verbose and out.strip():
                 print(out)
     if jobs or not os.path.exists(LIB):
         _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"], verbose)
+    if bind_stale or not os.path.exists(NATIVE):
+        lib = os.path.join(_torch(), "lib")
+        _run(["g++", "-shared", "-o", NATIVE, bind_obj, "-L" + os.path.dirname(LIB), "-lvxb", "-L" + lib,
+              "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib],
+             verbose)
     return LIB
 
 

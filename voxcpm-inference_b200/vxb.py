@@ -498,135 +498,47 @@ def residual_unit(w, w_type: int, C: int, d: int, x, batch: int, T: int, a1, dw,
 # ------------------------------------------------- language-model operators --
 # Tensors on one CUDA device, outputs given by the caller; sizes and strides
 # are the tensors' own (the last axis contiguous).  Work is enqueued on
-# `stream` or the device's current stream, on the tensors' device whichever
-# device is current.  A call that the C ABI or these checks refuse raises
-# VxbError(ERR_INVALID_ARGUMENT) and enqueues nothing.  (The checks are plain
-# comparisons: they run for every token of a stream, next to kernels of a few
-# microseconds.)
+# `stream` (a torch stream or a handle; None: the device's current stream), on
+# the tensors' device whichever device is current.  A call that the checks of
+# csrc/bind/native.cpp or the C ABI refuse raises
+# VxbError(ERR_INVALID_ARGUMENT) and enqueues nothing.
 
-_types: dict = {}
-
-
-def _types_of():
-    import torch
-
-    _types.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16,
-                   torch.float8_e4m3fn: TYPE_E4M3, torch.int32: "int32", torch.int64: "int64",
-                   torch.uint8: "uint8"})
-    return _types
+_native_module = None
 
 
-def _type(t):
-    """Type code of a tensor (a name for the index types, -1 for others)."""
-    return (_types or _types_of()).get(t.dtype, -1)
+def _native():
+    """Loads _vxb_native.so (fails loudly when it is missing)."""
+    global _native_module
+    if _native_module is None:
+        import importlib.machinery
+        import importlib.util
 
+        import torch  # noqa: F401  (the module's libraries)
 
-def _refuse(what: str):
-    raise VxbError(ERR_INVALID_ARGUMENT, what)
-
-
-def _is(t, what: str, shape: tuple, kind):
-    """Checks a tensor's shape, type and that its last axis is contiguous."""
-    if t.shape != shape:
-        _refuse(f"{what}: expected shape {list(shape)}, got {list(t.shape)}")
-    if (_types or _types_of()).get(t.dtype, -1) != kind:
-        _refuse(f"{what}: wrong type {t.dtype}")
-    if t.stride(-1) != 1 and shape[-1] > 1:
-        _refuse(f"{what}: the last axis must be contiguous")
-
-
-def _row_stride(t, N: int, C: int) -> int:
-    return t.stride(0) if N > 1 else C
-
-
-def _dims(t, what: str, n: int):
-    s = t.shape
-    if len(s) != n:
-        _refuse(f"{what}: expected {n} axes, got {len(s)}")
-    return s
-
-
-def _call(name: str, fn, args, tensors, stream):
-    """Calls a C entry on the tensors' device and stream (appended to args)."""
-    import torch
-
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            _refuse(f"{name}: tensors must be on one CUDA device")
-    if dev == torch.cuda.current_device():
-        if stream is None:
-            stream = torch._C._cuda_getCurrentRawStream(dev) or CUDA_STREAM_LEGACY
-        else:
-            stream = _stream(stream)
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream(stream))
-    if rc:
-        check(rc)
+        lib()
+        path = os.path.join(PKG, "lib", "_vxb_native.so")
+        if not os.path.exists(path):
+            raise VxbError(ERR_BACKEND, f"{path} not built (run voxcpm-inference_b200/build.py)")
+        loader = importlib.machinery.ExtensionFileLoader("_vxb_native", path)
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_vxb_native", loader))
+        loader.exec_module(m)
+        m.set_error(VxbError)
+        _native_module = m
+    return _native_module
 
 
 def rms_norm(x, weight, y, y_scale=None, residual=None, sum_out=None, eps: float = 1e-6, stream=None):
     """RMS norm of the rows of x [N, C] (float32, float16 or bfloat16), `residual`
     added first; the sum goes to `sum_out` (may be x or residual).  y: of x's
     type, or float8_e4m3fn with y_scale float32 [N, ceil(C / 128)]."""
-    N, C = shape = _dims(x, "x", 2)
-    kind, wkind, ykind = _type(x), _type(weight), _type(y)
-    _is(x, "x", shape, kind)
-    _is(weight, "weight", (C,), wkind)
-    _is(y, "y", shape, ykind)
-    rp = rs = sp = ss = cp = cs = 0
-    if residual is not None:
-        _is(residual, "residual", shape, kind)
-        rp, rs = residual.data_ptr(), _row_stride(residual, N, C)
-    if sum_out is not None:
-        _is(sum_out, "sum_out", shape, kind)
-        sp, ss = sum_out.data_ptr(), _row_stride(sum_out, N, C)
-    if y_scale is not None:
-        kb = (C + 127) // 128
-        _is(y_scale, "y_scale", (N, kb), TYPE_F32)
-        cp, cs = y_scale.data_ptr(), _row_stride(y_scale, N, kb)
-    _call("rms_norm", lib().vxb_rms_norm,
-          (kind, N, C, x.data_ptr(), _row_stride(x, N, C), rp, rs, sp, ss, wkind, weight.data_ptr(), eps, ykind,
-           y.data_ptr(), _row_stride(y, N, C), cp, cs), (x, weight, y, y_scale, residual, sum_out), stream)
+    (_native_module or _native()).rms_norm(x, weight, y, y_scale, residual, sum_out, eps, stream)
 
 
 def fp8_product(x, x_scale, w, w_scale, y, bias=None, stream=None):
     """y [N, M] = (x * x_scale) @ (w * w_scale)^T + bias for float8_e4m3fn x [N, K]
     and w [M, K], x_scale float32 [N, ceil(K / 128)] (one per token and block of
     128), w_scale float32 [ceil(M / 128), ceil(K / 128)], bias float32 [M]."""
-    N, K = _dims(x, "x", 2)
-    M = _dims(w, "w", 2)[0]
-    kb = (K + 127) // 128
-    _is(x, "x", (N, K), TYPE_E4M3)
-    _is(w, "w", (M, K), TYPE_E4M3)
-    _is(x_scale, "x_scale", (N, kb), TYPE_F32)
-    _is(w_scale, "w_scale", ((M + 127) // 128, kb), TYPE_F32)
-    ykind = _type(y)
-    _is(y, "y", (N, M), ykind)
-    if not w_scale.is_contiguous():
-        _refuse("w_scale must be contiguous")
-    if bias is not None:
-        _is(bias, "bias", (M,), TYPE_F32)
-    pitch = (K + 15) // 16 * 16  # of a single row
-    _call("fp8_product", lib().vxb_fp8_product,
-          (N, K, M, x.data_ptr(), _row_stride(x, N, pitch), x_scale.data_ptr(), _row_stride(x_scale, N, kb),
-           w.data_ptr(), _row_stride(w, M, pitch), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), ykind,
-           y.data_ptr(), _row_stride(y, N, M)), (x, x_scale, w, w_scale, y, bias), stream)
-
-
-def _heads(t, what: str, shape: tuple, kind):
-    _is(t, what, shape, kind)
-    s = t.stride()
-    return t.data_ptr(), s[0], s[1]
-
-
-def _angles(positions, inv_freq, N: int) -> int:
-    _is(positions, "positions", (N,), "int64")
-    half, = _dims(inv_freq, "inv_freq", 1)
-    _is(inv_freq, "inv_freq", (half,), TYPE_F32)
-    return 2 * half
+    (_native_module or _native()).fp8_product(x, x_scale, w, w_scale, y, bias, stream)
 
 
 def rotary(q, positions, inv_freq, q_out, k=None, k_out=None, interleaved: bool = False, factor: float = 1.0,
@@ -634,30 +546,7 @@ def rotary(q, positions, inv_freq, q_out, k=None, k_out=None, interleaved: bool 
     """Rotates the first 2 * len(inv_freq) dims of every head of q [N, Hq, D] (and k
     [N, Hk, D]) by positions [N] (int64) times inv_freq (float32), times
     `factor`, into q_out (and k_out); q_out may be q, k_out k."""
-    N, Hq, D = shape = _dims(q, "q", 3)
-    kind = _type(q)
-    R = _angles(positions, inv_freq, N)
-    Hk, kh, koh = 0, (0, 0, 0), (0, 0, 0)
-    if (k is None) != (k_out is None):
-        _refuse("k and k_out come together")
-    if k is not None:
-        Hk = _dims(k, "k", 3)[1]
-        kh, koh = _heads(k, "k", (N, Hk, D), kind), _heads(k_out, "k_out", (N, Hk, D), kind)
-    _call("rotary", lib().vxb_rotary,
-          (kind, N, Hq, Hk, D, R, 1 if interleaved else 0, factor, positions.data_ptr(), inv_freq.data_ptr(),
-           *_heads(q, "q", shape, kind), *_heads(q_out, "q_out", shape, kind), *kh, *koh),
-          (q, positions, inv_freq, q_out, k, k_out), stream)
-
-
-def _cache(k_cache, v_cache, Hk: int, D: int, kind):
-    """(pages, page size, strides of page, slot and head) of a cache pair."""
-    shape = _dims(k_cache, "k_cache", 4)
-    _is(k_cache, "k_cache", (shape[0], shape[1], Hk, D), kind)
-    _is(v_cache, "v_cache", shape, kind)
-    s = k_cache.stride()
-    if v_cache.stride() != s:
-        _refuse("k_cache and v_cache must have one set of strides")
-    return shape[0], shape[1], s[0], s[1], s[2]
+    (_native_module or _native()).rotary(q, positions, inv_freq, q_out, k, k_out, interleaved, factor, stream)
 
 
 def rotary_append(q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache, interleaved: bool = False,
@@ -665,18 +554,8 @@ def rotary_append(q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache, 
     """rotary() with the rotated keys and the values [N, Hk, D] written to the paged
     caches [pages, page_size, Hk, D] at slots [N] (int64; page * page_size +
     place, each its own; outside the cache: skipped)."""
-    N, Hq, D = shape = _dims(q, "q", 3)
-    kind = _type(q)
-    R = _angles(positions, inv_freq, N)
-    _is(slots, "slots", (N,), "int64")
-    Hk = _dims(k, "k", 3)[1]
-    kshape = (N, Hk, D)
-    _call("rotary_append", lib().vxb_rotary_append,
-          (kind, N, Hq, Hk, D, R, 1 if interleaved else 0, factor, positions.data_ptr(), slots.data_ptr(),
-           inv_freq.data_ptr(), *_heads(q, "q", shape, kind), *_heads(q_out, "q_out", shape, kind),
-           *_heads(k, "k", kshape, kind), *_heads(v, "v", kshape, kind), k_cache.data_ptr(), v_cache.data_ptr(),
-           *_cache(k_cache, v_cache, Hk, D, kind)),
-          (q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache), stream)
+    (_native_module or _native()).rotary_append(q, k, v, positions, slots, inv_freq, q_out, k_cache, v_cache,
+                                                interleaved, factor, stream)
 
 
 def rotary_frequencies(R: int, base: float = 10000.0, linear: float = 1.0, factors=None, original_length: int = 0,
@@ -709,45 +588,5 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale: 
     sqrt(D) if None; window > 0: a token sees the last `window` keys.
     `workspace`: a uint8 tensor of vxb_paged_attention_workspace bytes, else
     one is taken from torch's allocator on the call's stream."""
-    N, Hq, D = shape = _dims(q, "q", 3)
-    Hk = _dims(k_cache, "k_cache", 4)[2]
-    kind = _type(q)
-    pages, page_size, *strides = _cache(k_cache, v_cache, Hk, D, kind)
-    B, max_pages = _dims(block_table, "block_table", 2)
-    _is(block_table, "block_table", (B, max_pages), "int32")
-    _is(cu_q, "cu_q", (B + 1,), "int32")
-    _is(kv_len, "kv_len", (B,), "int32")
-    heads, oheads = _heads(q, "q", shape, kind), _heads(out, "out", shape, kind)
-    if workspace is not None:
-        _is(workspace, "workspace", workspace.shape, "uint8")
-    else:
-        workspace = _workspace(q, (N, B, Hq, Hk, D, max_pages, page_size), stream)
-    _call("paged_attention", lib().vxb_paged_attention,
-          (kind, N, B, Hq, Hk, D, *heads, k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *strides,
-           block_table.data_ptr(), block_table.stride(0), max_pages, cu_q.data_ptr(), kv_len.data_ptr(),
-           D ** -0.5 if scale is None else scale, window, *oheads,
-           0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel()),
-          (q, k_cache, v_cache, block_table, cu_q, kv_len, out, workspace), stream)
-
-
-def _workspace(q, extents, stream):
-    """The workspace of one paged_attention call, or None if it needs none."""
-    import torch
-
-    dev = q.get_device()
-    if dev < 0:
-        _refuse("paged_attention: tensors must be on one CUDA device")
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _workspace(q, extents, stream)
-    need = lib().vxb_paged_attention_workspace(*extents)
-    if need < 0:
-        _refuse(lib().vxb_last_error().decode())
-    if not need:
-        return None
-    if stream is None:
-        return torch.empty(need, dtype=torch.uint8, device=q.device)
-    # memory of the stream that uses it
-    s = torch.cuda.ExternalStream(stream, device=q.device) if isinstance(stream, int) else stream
-    with torch.cuda.stream(s):
-        return torch.empty(need, dtype=torch.uint8, device=q.device)
+    (_native_module or _native()).paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale, window,
+                                                  workspace, stream)
