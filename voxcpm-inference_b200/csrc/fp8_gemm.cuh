@@ -100,14 +100,17 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
-    float v;
-    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}\n"
-                 : "=f"(v)
-                 : "r"(saddr), "r"(rank)
-                 : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t saddr, uint32_t rank) {
+    float4 v;
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}\n"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        : "r"(saddr), "r"(rank)
+        : "memory");
     return v;
 }
+
+constexpr int kMaxSplit = 8;  // blocks of a cluster
 
 template <int BN, bool WROWS>
 struct Fp8Cfg {
@@ -125,10 +128,10 @@ struct Fp8Cfg {
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kBufCols = BN < 32 ? 32 : BN;
     static constexpr int kTmemCols = 2 * kBufCols;
-    // split: partial sums over the stages, [BN][128] (weights as rows) or [128][BN + 1] (tokens
-    // as rows), so that lanes along the output's fast axis read neighbouring words
-    static constexpr int kRedBytes = 128 * (BN + 1) * 4;
-    static __device__ __forceinline__ int red_at(int row, int col) { return WROWS ? col * 128 + row : row * (BN + 1) + col; }
+    // split: partial sums over the stages, [BN][128] (weights as rows) or [128][BN + 4] (tokens
+    // as rows), so that four outputs next to each other are four neighbouring words
+    static constexpr int kRedBytes = 128 * (BN + 4) * 4;
+    static __device__ __forceinline__ int red_at(int row, int col) { return WROWS ? col * 128 + row : row * (BN + 4) + col; }
     static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + 1024 + 512;
     static_assert(kRedBytes <= kStages * kStageBytes, "partial sums fit the drained stages");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
@@ -422,16 +425,26 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             const int r0 = static_cast<int>(tile0 % args.row_tiles) * 128;
             const int64_t c0 = tile0 / args.row_tiles * BN;
             const uint32_t red = smem_u32(stages);
-            // rank's share of the tile, a warp's lanes along the output's fast axis
-            for (int i = rank * static_cast<int>(blockDim.x) + threadIdx.x; i < BN * 128; i += split * blockDim.x) {
-                const int c = WROWS ? i >> 7 : i % BN, rr = WROWS ? i & 127 : i / BN;
+            // rank's share of the tile, four outputs of a row at a time
+            constexpr int kQuads = WROWS ? 32 : BN / 4;  // of a row of outputs
+            for (int i = rank * static_cast<int>(blockDim.x) + threadIdx.x; i < BN * 32; i += split * blockDim.x) {
+                const int c = WROWS ? i / kQuads : i % kQuads * 4, rr = WROWS ? i % kQuads * 4 : i / kQuads;
                 const int64_t n = WROWS ? c0 + c : r0 + rr;
                 const int64_t m = WROWS ? r0 + rr : c0 + c;
                 if (n >= args.N || m >= args.M) continue;
-                float v = 0.f;
-                for (int p = 0; p < split; ++p) v += ld_cluster_f32(red + Cfg::red_at(rr, c) * 4, p);
-                if (args.bias) v += args.bias[m];
-                store_out(args.y, n * args.y_stride + m, v, args.out_type);
+                float4 part[kMaxSplit];
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p)
+                    part[p] = p < split ? ld_cluster_f32x4(red + Cfg::red_at(rr, c) * 4, p) : make_float4(0.f, 0.f, 0.f, 0.f);
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p)
+                    v[0] += part[p].x, v[1] += part[p].y, v[2] += part[p].z, v[3] += part[p].w;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (m + x < args.M)
+                        store_out(args.y, n * args.y_stride + m + x, v[x] + (args.bias ? args.bias[m + x] : 0.f),
+                                  args.out_type);
             }
         }
         __syncwarp();

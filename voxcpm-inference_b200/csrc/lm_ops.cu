@@ -276,7 +276,7 @@ int launch_fp8(const Fp8Operands& o, Fp8GemmArgs a, int dev, cudaStream_t st) {
     // fewer tiles than SMs: K is shared by the blocks of a cluster, each with two k blocks at least
     const int sms = num_sms(dev);
     a.split = 1;
-    while (Cfg::kSplits && a.split < 8 && a.tiles * a.split * 2 <= sms && a.kb >= a.split * 4) a.split *= 2;
+    while (Cfg::kSplits && a.split < kMaxSplit && a.tiles * a.split * 2 <= sms && a.kb >= a.split * 4) a.split *= 2;
     CUtensorMap tx, tw, ty = {};
     if (Cfg::kTmaOut) {
         const int es = a.out_type == kOutF32 ? 4 : 2;
@@ -320,10 +320,22 @@ extern "C" int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x
         a.out_type = y_type == VXB_TYPE_F32 ? kOutF32 : y_type == VXB_TYPE_F16 ? kOutF16 : kOutBF16;
         const Fp8Operands o{x, w, x_stride, w_stride};
         cudaStream_t st = static_cast<cudaStream_t>(stream);
+        // Few tokens: weights as rows, so that a tile's 128 rows are all in use and the tokens
+        // set its width.  So too where there are more tokens but few tiles of 128 x 128
+        // (256 x 1024 -> 64: 4.2 us against 5.9; 77 x 1536 -> 1001: 5.5 against 6.5; with 32
+        // such tiles the other way round, 128 x 4096 -> 4096: 13.6 against 9.8): 64 tokens wide
+        // if that fills the SMs with K split, else 32.  256 outputs wide where that fills them.
+        const int sms = num_sms(dev);
+        const int64_t rows = (int64_t(M) + 127) / 128;
         if (N <= 16) return launch_fp8<16, true>(o, a, dev, st);
         if (N <= 32) return launch_fp8<32, true>(o, a, dev, st);
         if (N <= 64) return launch_fp8<64, true>(o, a, dev, st);
-        if ((N + 127) / 128 * ((M + 255) / 256) >= num_sms(dev)) return launch_fp8<256, false>(o, a, dev, st);
+        if ((N + 127) / 128 * rows <= 16) {
+            const int64_t most = (N + 63) / 64 * rows * std::min(kMaxSplit, std::max(1, kb / 2));
+            if (most * 5 >= sms * 4) return launch_fp8<64, true>(o, a, dev, st);
+            return launch_fp8<32, true>(o, a, dev, st);
+        }
+        if ((N + 127) / 128 * ((M + 255) / 256) >= sms) return launch_fp8<256, false>(o, a, dev, st);
         return launch_fp8<128, false>(o, a, dev, st);
     });
 }
