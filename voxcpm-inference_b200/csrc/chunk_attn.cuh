@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     uint64_t* empty = full + R;
     uint64_t* q_bar = empty + R;
     uint64_t* s_full = q_bar + 1;    // [2] scores of a tile ready
-    uint64_t* p_full = s_full + 2;   // [2] P written
-    uint64_t* o_done = p_full + 2;   // [2] O updated
+    uint64_t* p_full = s_full + 2;   // [2][2] a half of P written
+    uint64_t* o_done = p_full + 4;   // [2] O updated
     uint64_t* clear = o_done + 2;    // [R] the slot's tile has been looked at (and cleared)
     uint64_t* end_bar = clear + R;   // every tile has been looked at
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(end_bar + 1);
@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         mbar_init(q_bar, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_done[i], 1);
         }
         mbar_init(end_bar, 2);
@@ -298,13 +299,17 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                 if (ok && j + 1 < steps) ok = wait(&clear[ik % R], (ik / R) & 1, kErrWaitFull);
                 const uint32_t vb = kLowV | (ring_addr + (iv % R) * (Cfg::kTileBytes / 16));
                 for (int i = 0; i < tiles && ok; ++i) {
-                    ok = wait(&p_full[i], j & 1, kErrWaitAccum);
-                    if (!ok) break;
-                    tc_fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < kCkStep / 16; ++kk)  // 16 keys: 8 TMEM columns of P, 2 KB of V rows
-                        umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vb + kk * (2048 / 16), idesc_o,
-                                (j | kk) != 0, leader);
+                    for (int half = 0; half < 2; ++half) {  // (the product starts on the first half of P)
+                        ok = ok && wait(&p_full[2 * i + half], j & 1, kErrWaitAccum);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)  // 16 keys: 8 TMEM columns of P, 2 KB of V rows
+                            umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vb + kk * (2048 / 16), idesc_o,
+                                    (j | kk) != 0, leader);
+                    }
+                    if (!ok) break;
                     umma_commit_by(&o_done[i], leader);
                     if (i == tiles - 1) umma_commit_by(&empty[iv % R], leader);
                     // (in order behind the product that reads P, which these scores overwrite)
@@ -406,13 +411,13 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                     if (key > pos || key <= lo || !((there >> (c >> 4)) & 1)) s[c] = kNegInf;
                 }
             }
-            float t0 = s[0], t1 = s[1];
+            float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 2; c < 128; c += 4) {
-                t0 = fmaxf(t0, fmaxf(s[c], s[c + 1]));
-                if (c + 2 < 128) t1 = fmaxf(t1, fmaxf(s[c + 2], s[c + 3]));
-            }
-            const float top = fmaxf(t0, t1);
+            for (int c = 4; c < 124; c += 8)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) t4[x] = fmaxf(t4[x], fmaxf(s[c + x], s[c + 4 + x]));
+            const float top = fmaxf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])),
+                                    fmaxf(fmaxf(s[124], s[125]), fmaxf(s[126], s[127])));
             // rescale if some row of the warp has outgrown its m
             const bool grow = m == kNegInf ? top > kNegInf : (top - m) * scale > kAttnLazy;
             if (__any_sync(0xffffffffu, grow)) {
@@ -454,12 +459,14 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                     p[x] = Mma::pack(w.x, w.y);
                 }
                 tmem_st16(ts + c / 2, p);
+                if (c & 32) {  // 64 keys are written: the product with V starts on them
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * i + c / 64]);
+                }
             }
             l += (sum.x + sum.y) + (sum2.x + sum2.y);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i]);
         }
         if (n > 0 && ok) {
             ok = mbar_wait(&o_done[i], (n - 1) & 1, abort_flag, nullptr, kErrWaitAccum);
