@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     uint8_t* sq = smem + S * 2 * Cfg::kTileBytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(sq + Cfg::kQBytes);
     uint64_t* empty = full + S;
+    volatile uint32_t* there = reinterpret_cast<volatile uint32_t*>(empty + S);  // [S] pages of the slot's step
     __shared__ AttnTile sh_tile;
     __shared__ int sh_poison;
     __shared__ int sh_abort;
@@ -283,7 +284,14 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
                 ok = mbar_wait(&empty[slot], ((i / S) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], 2 * Cfg::kTileBytes);
+                // bit g: keys 16 g .. 16 g + 15 of the step lie in a page
+                const uint32_t valid = __ballot_sync(0xffffffffu, bx < bps && pg >= 0 && pg < a.pages);
+                const uint32_t groups = __ballot_sync(
+                    0xffffffffu, lane < kStep / 16 && ((valid >> ((lane * 16 / box) * H * 2 & 31)) & 1));
+                if (lane == 0) {
+                    there[slot] = groups;
+                    mbar_arrive_expect_tx(&full[slot], 2 * Cfg::kTileBytes);
+                }
                 __syncwarp();
                 if (bx < bps) {
                     if (pg < 0 || pg >= a.pages) pg = static_cast<int>(a.pages);  // past the cache: zeros
@@ -346,12 +354,6 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         for (int k = 0; k < DP / 16; ++k)
             ldsm_x4(qf[kQRegs ? k : 0], smem_u32(sq) + attn_off<Cfg::kRows>(lane & 15, 2 * k + (lane >> 4)));
     }
-    auto is_absent = [&](int step) {  // does this lane's key (of the warp's) lie in no page?
-        const int j = step * kStep + warp * 16 * KW + (lane & (16 * KW - 1));
-        const int pg = j < key_hi ? table[j >> a.page_shift] : -1;
-        return pg < 0 || pg >= a.pages;
-    };
-    bool gone = warp < 4 && my_lo < my_hi && is_absent(my_lo);
     bool ok = true;
     for (int step = warp < 4 ? my_lo : my_hi; step < my_hi; ++step) {
         const int it = step - my_lo, slot = it % S;
@@ -360,13 +362,13 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         const int j0 = step * kStep + warp * 16 * KW;  // this warp's keys
         // does every row see all of the warp's keys?
         bool whole = j0 + 16 * KW - 1 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
-        // bit i: key j0 + i lies in no page
-        const uint32_t absent = __ballot_sync(0xffffffffu, gone);  // (16 keys: in both halves)
-        whole = whole && absent == 0;
-        gone = step + 1 < my_hi && is_absent(step + 1);  // (of the next step: its entry is here in time)
         ok = mbar_wait(&full[slot], (it / S) & 1, abort_flag, nullptr, kErrWaitFull);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        // bit i: key j0 + i lies in no page
+        const uint32_t in = there[slot] >> (warp * KW);
+        const uint32_t absent = (in & 1 ? 0 : 0xffffu) | (KW > 1 && !(in & 2) ? 0xffff0000u : 0);
+        whole = whole && absent == 0;
         if (!whole) {
             // A key that some row does not see has weight 0 there, but 0 * inf is NaN: non-finite
             // values leave the tile and are added at the end to the rows that see them.
