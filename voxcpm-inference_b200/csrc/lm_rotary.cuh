@@ -11,7 +11,10 @@
 // subtracted the rest is rounded to fp32 (error below 2^-25 turns).
 //
 // HBM bound: q, k, v read and written once.  A block computes its tokens'
-// sines and cosines once into shared memory, for all heads; then every thread
+// sines and cosines once into shared memory, for all heads; small blocks (128
+// threads, 4 tokens) so that others move data meanwhile (16381 tokens of 32 + 16
+// heads of 128: 68 us, 5.9 TB/s; 256 threads and 8 tokens with four vectors in
+// flight a thread 76 us, with two 69 us, 2 tokens 91 us).  Then every thread
 // moves 16-byte vectors (VEC elements; element by element where a stride or an
 // extent does not allow it).
 #pragma once
@@ -20,9 +23,9 @@
 
 namespace vxb {
 
-constexpr int kRotTokens = 8;    // tokens per block at most
+constexpr int kRotTokens = 4;    // tokens per block at most
 constexpr int kRotMaxR = 256;
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 
 struct HeadsView {               // [N][heads][D], D contiguous
     void* p;
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     // by adding the block's stride in these three digits: no divisions.
     constexpr int kStep = INTER ? (VEC > 1 ? VEC : 2) : VEC;
     constexpr int kLoads = INTER ? (VEC > 1 ? 1 : 2) : 2;  // vectors of an item
-    constexpr int kAhead = 4;                              // items whose loads are in flight
+    constexpr int kAhead = 2;                              // items whose loads are in flight
     using V = typename VecOf<T, VEC>::type;
     const int pair_items = INTER ? a.R / kStep : half / kStep;
     const int head_items = pair_items + (a.D - a.R) / VEC;
