@@ -381,7 +381,7 @@ VXB_API int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R,
  * [pages][page_size][Hk][D] (one set of strides for both).  A table entry
  * outside [0, pages) makes its keys unseen (a page given back by a sliding
  * window); entries past a sequence's keys are not read, kv_len beyond
- * max_pages * page_size is cut to it, and values that no token sees, non-finite
+ * max_pages * page_size (below 2^30) is cut to it, and values that no token sees, non-finite
  * ones too, have no effect.  Rows of q and out outside every sequence are not
  * touched.  type F16 or BF16; D % 8 == 0, D <= 128; page_size a power of two
  * >= 16; q and cache bases and strides multiples of 16 bytes.  `workspace`:

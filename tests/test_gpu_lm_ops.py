@@ -514,6 +514,39 @@ def test_attention_lengths_out_of_range_are_cut(vxb):
     assert torch.equal(b.out[0], ref[0]) and (b.out[1] == 5).all()
 
 
+@pytest.mark.parametrize("q_len", [6, 100])
+def test_attention_widest_window_is_none(vxb, q_len):
+    """Fewer keys than new tokens: the first tokens stand before key 0, and a window of 2^31 - 1
+    reaches no further than any other."""
+    b = Batch([q_len], [q_len - 4], 8, 2, 64, 16, torch.bfloat16)
+    b.run(vxb)
+    b.check()
+    ref = b.out.clone()
+    for window in (2 ** 31 - 1, 2 ** 30, b.table.shape[1] * 16):
+        b.window = window
+        b.out.fill_(5.0)
+        b.run(vxb)
+        assert torch.equal(b.out, ref)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+def test_attention_row_ranges_that_overlap_stay_in_bounds(vxb, heads):
+    """Not sequences, so their rows' values mean nothing; the rows of proper ones and those of none do."""
+    b = Batch([40, 20, 20, 20], [60, 50, 45, 70], heads, 1, 64, 16, torch.bfloat16, tail=4)
+    b.cu[2] = 30  # the second ends before it starts, the third begins inside the first
+    b.run(vxb)
+    torch.cuda.synchronize()
+    assert torch.isfinite(b.out).all() and (b.out[100:] == 5).all()
+
+
+def test_axes_of_one_element_have_any_stride(vxb):
+    b = Batch([1], [40], 4, 1, 64, 16, torch.bfloat16)
+    b.k, b.v = (t.as_strided(t.shape, (t.stride(0), t.stride(1), 3, 1)) for t in (b.k, b.v))
+    b.q = b.q.as_strided(b.q.shape, (7, b.q.stride(1), 1))
+    b.run(vxb)
+    b.check()
+
+
 @pytest.mark.parametrize("q_len", [1, 100])
 def test_attention_offsets_beyond_32_bits(vxb, q_len):
     """A cache of 2.2e9 elements; the pages in use are its first and last."""

@@ -83,7 +83,7 @@ ATTN = dict(type=vxb.TYPE_BF16, N=4, B=2, Hq=8, Hk=2, D=64, q=P, qt=512, qh=64, 
 @pytest.mark.parametrize("change", [
     dict(type=vxb.TYPE_F32), dict(type=vxb.TYPE_E4M3), dict(N=-1), dict(B=-1), dict(Hq=7), dict(Hk=0), dict(D=60),
     dict(D=136), dict(D=0), dict(page=8), dict(page=24), dict(page=0), dict(pages=-1), dict(mp=-1),
-    dict(mp=2 ** 27, ts=2 ** 27), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
+    dict(mp=2 ** 27, ts=2 ** 27), dict(mp=2 ** 26, ts=2 ** 26), dict(N=2 ** 30 + 1), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
     dict(out=None), dict(kc=None), dict(vc=None), dict(table=None), dict(cu=None), dict(kv=None), dict(ts=3),
     dict(q=P + 8), dict(kc=P + 2), dict(qt=513), dict(qh=60), dict(ps=2049), dict(ss=129), dict(hs=63),
     dict(out=P + 1), dict(table=P + 2)])

@@ -93,6 +93,14 @@ struct Call {
         }
         return v;
     }
+    bool truth(int i, const char* what) {
+        const int v = PyObject_IsTrue(args[i]);
+        if (v < 0) {
+            PyErr_Clear();
+            refuse(std::string(op) + ": " + what + " must be true or false");
+        }
+        return v != 0;
+    }
     long integer(int i, const char* what) {
         int over = 0;
         const long v = PyLong_AsLongAndOverflow(args[i], &over);
@@ -189,11 +197,15 @@ void fp8_product(Call& c) {
                           type_of(y), ptr(y), row_stride(y, N, M), d.stream));
 }
 
+// Strides of [N][heads][D]; an axis of one element has whatever stride fits.
 struct Heads {
     void* p = nullptr;
     int64_t token = 0, head = 0;
     Heads() = default;
-    explicit Heads(const at::Tensor& t) : p(ptr(t)), token(t.stride(0)), head(t.stride(1)) {}
+    explicit Heads(const at::Tensor& t)
+        : p(ptr(t)),
+          token(t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2)),
+          head(t.size(1) > 1 ? t.stride(1) : t.size(2)) {}
 };
 
 int checked_int(const char* op, int64_t v) {
@@ -220,7 +232,7 @@ void rotary(Call& c) {
     }
     for (const at::Tensor* t : {&q, &pos, &f, &qo, k, ko})
         if (t) c.on_device(*t);
-    const int inter = PyObject_IsTrue(c.args[6]) == 1;
+    const int inter = c.truth(6, "interleaved");
     const float factor = static_cast<float>(c.number(7, "factor"));
     const Heads hq(q), hqo(qo), hk = k ? Heads(*k) : Heads(), hko = ko ? Heads(*ko) : Heads();
     OnDevice d(c, c.args[8]);
@@ -240,11 +252,15 @@ struct Cache {
             refuse(std::string(c.op) + ": k_cache: expected [.., .., " + std::to_string(Hk) + ", " + std::to_string(D) +
                    "], got " + shape_text(kc.sizes()));
         const at::Tensor& vc = c.of(iv, "v_cache", 4, type);
-        if (vc.sizes() != kc.sizes() || vc.strides() != kc.strides())
-            refuse(std::string(c.op) + ": k_cache and v_cache must have one shape and one set of strides");
+        if (vc.sizes() != kc.sizes()) refuse(std::string(c.op) + ": k_cache and v_cache must have one shape");
+        for (int i = 0; i < 3; ++i)
+            if (kc.size(i) > 1 && kc.stride(i) != vc.stride(i))
+                refuse(std::string(c.op) + ": k_cache and v_cache must have one set of strides");
         k = &kc, v = &vc;
         pages = kc.size(0), page = kc.size(1);
-        page_stride = kc.stride(0), slot_stride = kc.stride(1), head_stride = kc.stride(2);
+        head_stride = Hk > 1 ? kc.stride(2) : D;
+        slot_stride = page > 1 ? kc.stride(1) : Hk * D;
+        page_stride = pages > 1 ? kc.stride(0) : page * Hk * D;
     }
 };
 
@@ -263,7 +279,7 @@ void rotary_append(Call& c) {
     const at::Tensor& qo = c.of(6, "q_out", {N, Hq, D}, type);
     const Cache m(c, 7, 8, Hk, D, type);
     for (const at::Tensor* t : {&q, &k, &v, &pos, &slots, &f, &qo, m.k, m.v}) c.on_device(*t);
-    const int inter = PyObject_IsTrue(c.args[9]) == 1;
+    const int inter = c.truth(9, "interleaved");
     const float factor = static_cast<float>(c.number(10, "factor"));
     const Heads hq(q), hqo(qo), hk(k), hv(v);
     OnDevice d(c, c.args[11]);

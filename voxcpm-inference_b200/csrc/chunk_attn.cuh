@@ -135,6 +135,7 @@ __device__ __forceinline__ AttnTile find_long_tile(const AttnArgs& a, int64_t sl
             *sh = t;
         }
     }
+    fence_proxy_async_smem();  // (`work` lies where TMA writes next)
     __syncthreads();
     return *sh;
 }

@@ -457,13 +457,14 @@ int launch_attn(const AttnArgs& a, const AttnPlan& p, int dev, cudaStream_t st) 
 }
 
 int check_attn(const char* op, int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size) {
-    if (N < 0 || N > kMaxRows || B < 0 || B > (1 << 24)) return bad(op, "bad token or sequence count");
+    // (positions and windows are 32-bit differences of these)
+    if (N < 0 || N > (1 << 30) || B < 0 || B > (1 << 24)) return bad(op, "bad token or sequence count");
     if (Hk < 1 || Hq < 1 || Hq % Hk || Hq > 4096) return bad(op, "query heads must be a multiple of key heads");
     if (D < 8 || D % 8 || D > kAttnMaxD) return bad(op, "head width must be a multiple of 8, 8..128");
     if (page_size < 16 || (page_size & (page_size - 1)) || page_size > (1 << 20))
         return bad(op, "page size must be a power of two, 16 at least");
-    if (max_pages < 0 || int64_t(max_pages) * page_size >= (int64_t(1) << 31) - 4096)
-        return bad(op, "a table row must cover less than 2^31 keys");
+    if (max_pages < 0 || int64_t(max_pages) * page_size >= (int64_t(1) << 30))
+        return bad(op, "a table row must cover less than 2^30 keys");
     return VXB_OK;
 }
 
@@ -520,7 +521,8 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         a.table = block_table, a.table_stride = table_stride, a.cu_q = cu_q, a.kv_len = kv_len;
         a.N = N, a.pages = pages, a.B = B, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk, a.D = D;
         // (a cache without pages: no key is seen, nothing is loaded)
-        a.page_size = page_size, a.max_pages = pages ? max_pages : 0, a.window = window;
+        a.page_size = page_size, a.max_pages = pages ? max_pages : 0;
+        a.window = window < int64_t(max_pages) * page_size ? window : 0;  // (as wide as the table: none)
         while ((1 << a.page_shift) < page_size) ++a.page_shift;
         // (a scale of 0 weighs every key alike; the smallest normal number does too, and keeps
         // a masked score, -inf, times it -inf)

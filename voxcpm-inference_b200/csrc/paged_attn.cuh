@@ -159,12 +159,23 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int64_t slot, i
         __syncthreads();
         return t;
     }
-    if (threadIdx.x == 0) sh->b = -1;
+    // (the first sequence that claims the slot has it: with row ranges that overlap, which
+    // are not sequences, two could)
+    if (threadIdx.x == 0) sh->b = INT32_MAX;
     __syncthreads();
     for (int b = threadIdx.x; b < a.B; b += blockDim.x)
-        if (tile_of(a, b, slot, TT, &t)) *sh = t;
+        if (tile_of(a, b, slot, TT, &t)) {
+            atomicMin(&sh->b, b);
+            break;
+        }
     __syncthreads();
-    return *sh;
+    const int b = sh->b;
+    if (b == INT32_MAX) {
+        t.b = -1;
+    } else {
+        tile_of(a, b, slot, TT, &t);
+    }
+    return t;
 }
 
 template <typename T, int DP, int MT, int KW>
