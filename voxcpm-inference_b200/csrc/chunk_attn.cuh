@@ -9,9 +9,14 @@
 //   O += P V   (A operand from TMEM, fp32 accumulator in TMEM)
 // A warpgroup owns a tile's softmax, one row per thread: the maximum and the
 // sum need no exchange.  While one tile's softmax runs, the tensor cores work
-// on the other tile, so 2 * 2 products of 128 x 128 x D hide under the
-// exponentials of 2 * 128 * 128 scores and the other way round; both take
-// about the same time at D = 128 (16 exponentials per clock and SM).
+// on the other tile; the product with V starts on the first 64 keys' weights.
+//
+// Bound (one B200, 4 chunks of up to 2048 tokens over up to 8192 keys, 32 / 8
+// heads of 128: 428 us, 949 TFLOP/s; 242 us at the measured dense rate): a step
+// of both tiles takes about 4100 clocks, the MMAs 2100 and the exponentials of
+// the special-function unit 2048 of them; a tile's softmax takes 2200, and its
+// hand-over to the MMA warp and back 700.  TMEM has no room for a third score
+// buffer beside two outputs of 128 columns.
 //
 // m is the running maximum only loosely: O and the sum are rescaled when the
 // maximum has grown by more than 2^8 since the last time (P stays below 2^8,
@@ -48,8 +53,8 @@ struct ChunkCfg {
 
 // One tcgen05.mma, kind::f16, issued by the lane whose `leader` is set of a warp
 // that runs together: in a branch of one lane the operands would have to be
-// carried to uniform registers for every instruction (about 65 clocks each,
-// more than the product of 64 columns takes).  The matrix descriptors are
+// carried to uniform registers for every instruction (479 us against 462 for the
+// case above, before its tiles were ordered).  The matrix descriptors are
 // {address >> 4 | leading offset >> 4 << 16, kDescHigh}: 32-bit arithmetic.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride offset 1024, version, 128-byte swizzle
 
