@@ -579,12 +579,36 @@ def test_operators_on_another_stream(vxb):
     torch.cuda.synchronize()
     ref = b.out.clone()
     s = torch.cuda.Stream()
-    for stream in (s, s.cuda_stream):
+    for stream in (s, s.cuda_stream, torch.cuda.default_stream(), 0):
         b.out.fill_(5.0)
         s.wait_stream(torch.cuda.current_stream())
         b.run(vxb, stream=stream)
-        s.synchronize()
+        torch.cuda.synchronize()
         assert torch.equal(b.out, ref)
+
+
+def test_products_and_norms_on_two_streams_at_once(vxb):
+    """Calls that share the device keep apart: clusters, tensor memory and staging are their own."""
+    sets = []
+    for i, (N, K, M) in enumerate(((9, 4096, 512), (600, 1024, 2000), (200, 2048, 640), (3000, 512, 1536))):
+        x, xs = codes(10 * i, N, K, 1)
+        w, ws = codes(10 * i + 5, M, K, 128)
+        y = torch.empty(N, M, dtype=torch.bfloat16, device="cuda")
+        vxb.fp8_product(x, xs, w, ws, y)
+        n = torch.empty_like(y)
+        vxb.rms_norm(y, torch.ones(M, device="cuda"), n)
+        sets.append((x, xs, w, ws, torch.ones(M, device="cuda"), y.clone(), n.clone(), torch.empty_like(y), torch.empty_like(n)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(8):
+        for i, (x, xs, w, ws, g, ry, rn, y, n) in enumerate(sets):
+            st = streams[(i + turn // 4) % 2]
+            st.wait_stream(streams[(i + turn // 4 + 1) % 2] if turn % 4 == 0 else st)
+            vxb.fp8_product(x, xs, w, ws, y, stream=st)
+            vxb.rms_norm(y, g, n, stream=st)
+    torch.cuda.synchronize()
+    for x, xs, w, ws, g, ry, rn, y, n in sets:
+        assert torch.equal(y, ry) and torch.equal(n, rn)
 
 
 def test_two_captured_graphs_and_an_eager_call(vxb):
