@@ -180,7 +180,7 @@ def product_case(vxb, N, K, M, dtype, bias=True):
 @pytest.mark.parametrize("N,K,M", [
     (1, 16, 1), (1, 128, 128), (2, 1024, 64), (16, 1536, 1000), (17, 144, 129), (31, 4096, 512), (33, 2048, 255),
     (64, 8192, 384), (65, 128, 64), (77, 1536, 1001), (128, 1008, 256), (129, 256, 130), (200, 4096, 1024),
-    (1, 8192, 8192), (700, 512, 7000), (2500, 384, 2056), (1281, 640, 4100)])
+    (1, 8192, 8192), (1, 4096, 4096), (1, 1040, 4099), (2, 2048, 129), (2, 16, 3), (3, 528, 70), (700, 512, 7000), (2500, 384, 2056), (1281, 640, 4100)])
 def test_fp8_product(vxb, N, K, M, dtype):
     product_case(vxb, N, K, M, dtype)
 
@@ -191,7 +191,7 @@ def test_fp8_product_types_and_bias(vxb):
         product_case(vxb, 150, 512, 300, dtype, bias=True)
 
 
-@pytest.mark.parametrize("N", [3, 50, 150])
+@pytest.mark.parametrize("N", [1, 2, 3, 50, 150])
 def test_fp8_product_strided(vxb, N):
     K, M = 400, 200
     x, xs = codes(1, N, K, 1)
@@ -217,8 +217,21 @@ def test_fp8_product_non_finite_stays_in_its_row_and_column(vxb):
         assert torch.equal(~torch.isfinite(y), bad)
 
 
+def test_fp8_product_of_one_token_with_non_finite_codes(vxb):
+    x, xs = codes(1, 2, 512, 1)
+    w, ws = codes(5, 260, 512, 128)
+    x.view(torch.uint8)[1, 300] = 0xFF  # NaN
+    w.view(torch.uint8)[150, 20] = 0x7F
+    ws[0, 2] = float("inf")
+    y = torch.empty(2, 260, device="cuda")
+    vxb.fp8_product(x, xs, w, ws, y)
+    bad = torch.zeros(2, 260, dtype=torch.bool, device="cuda")
+    bad[1], bad[:, 150], bad[:, :128] = True, True, True
+    assert torch.equal(~torch.isfinite(y), bad)
+
+
 def test_fp8_product_repeats_bit_for_bit(vxb):
-    for N, K, M in ((7, 4096, 640), (100, 2048, 640), (600, 1024, 2000)):
+    for N, K, M in ((1, 1024, 700), (7, 4096, 640), (100, 2048, 640), (600, 1024, 2000)):
         x, xs = codes(1, N, K, 1)
         w, ws = codes(5, M, K, 128)
         a, b = (torch.empty(N, M, device="cuda") for _ in range(2))

@@ -22,7 +22,7 @@
 // share of the columns over distributed shared memory, in rank order (the
 // result does not depend on timing).
 //
-// Bounds and measurements (one B200).  Few tokens: 1 x 1024 -> 4096 4.4 us, a
+// Bounds and measurements (one B200).  Few tokens: 4 x 1024 -> 4096 4.6 us, a
 // chain of launch, TMA, MMA and join; 1 x 8192 -> 8192 16.9 us, 4.0 TB/s of
 // weights.  Many: 8192 x 4096 -> 8192 293 us (1880 TFLOP/s; the MMAs are busy
 // 45 % of the time): 203 us with the scaled additions left out, 177 us with the

@@ -12,6 +12,7 @@
 
 #include "chunk_attn.cuh"
 #include "fp8_gemm.cuh"
+#include "fp8_gemv.cuh"
 #include "host.h"
 #include "lm_norm.cuh"
 #include "lm_rotary.cuh"
@@ -291,6 +292,14 @@ int launch_fp8(const Fp8Operands& o, Fp8GemmArgs a, int dev, cudaStream_t st) {
     return VXB_OK;
 }
 
+template <int NT>
+int launch_fp8_gemv(const Fp8Operands& o, const Fp8GemmArgs& a, cudaStream_t st) {
+    constexpr int rows = kGemvRows * kGemvThreads / 32;
+    CUDA_TRY(launch_pdl(fp8_gemv_kernel<NT>, dim3((a.M + rows - 1) / rows), dim3(kGemvThreads), 0, st,
+                        static_cast<const uint8_t*>(o.x), o.x_stride, static_cast<const uint8_t*>(o.w), o.w_stride, a));
+    return VXB_OK;
+}
+
 }  // namespace
 
 extern "C" int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x_stride, const float* x_scale,
@@ -327,6 +336,10 @@ extern "C" int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x
         // if that fills the SMs with K split, else 32.  256 outputs wide where that fills them.
         const int sms = num_sms(dev);
         const int64_t rows = (int64_t(M) + 127) / 128;
+        // One or two tokens and a few MB of weights in rows of at most 4096: no tensor cores, no
+        // chain of set-up (measurements beside the kernel).
+        if (N == 1 && K <= 4096 && int64_t(K) * M <= (1 << 24)) return launch_fp8_gemv<1>(o, a, st);
+        if (N == 2 && K <= 2048 && int64_t(K) * M <= (1 << 23)) return launch_fp8_gemv<2>(o, a, st);
         if (N <= 16) return launch_fp8<16, true>(o, a, dev, st);
         if (N <= 32) return launch_fp8<32, true>(o, a, dev, st);
         if (N <= 64) return launch_fp8<64, true>(o, a, dev, st);
