@@ -288,9 +288,10 @@ def test_rotary(vxb, N, Hq, Hk, D, R, inter, dtype):
 
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("order", ["slots first", "heads first", "joint"])
-def test_rotary_append(vxb, inter, order):
-    N, Hq, Hk, D, R, page, pages = 50, 8, 2, 64, 48, 16, 9
-    dt = torch.bfloat16
+@pytest.mark.parametrize("dt,D,R,page", [(torch.bfloat16, 64, 48, 16), (torch.float32, 64, 64, 16),
+                                         (torch.float16, 20, 10, 10), (torch.float32, 6, 2, 1)])
+def test_rotary_append(vxb, inter, order, dt, D, R, page):
+    N, Hq, Hk, pages = 50, 8, 2, 9 if page > 1 else 140
     qkv = randn(1, N, (Hq + 2 * Hk) * D, dtype=dt)  # rows of one projection
     q, k, v = (t.view(N, -1, D) for t in qkv.split([Hq * D, Hk * D, Hk * D], 1))
     if order == "heads first":
@@ -495,6 +496,40 @@ def test_attention_non_finite_keys_reach_only_tokens_that_see_them(vxb):
     want = torch.zeros(30, 4, dtype=torch.bool, device="cuda")
     want[20:, :2] = True
     assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("q_len", [[1, 1, 1], [30, 1, 9], [200, 70, 90]])
+def test_attention_rows_before_the_first_sequence_and_shared_pages(vxb, q_len):
+    """Sequences may start behind row 0 of q, and may share pages (a common prompt)."""
+    b = Batch(q_len, [n + 64 for n in q_len], 8, 2, 64, 16, torch.bfloat16)
+    for i in (1, 2):  # the first 48 keys are sequence 0's
+        b.table[i, :3] = b.table[0, :3]
+        for x in (0, 1):
+            b.keys[i][x][:48] = b.keys[0][x][:48]
+    b.run(vxb)
+    b.check()
+    ref = b.out.clone()
+    b.q = torch.cat([randn(9, 5, 8, 64, dtype=torch.bfloat16), b.q])
+    b.out = torch.full_like(b.q, 5.0)
+    b.cu += 5
+    b.run(vxb)
+    assert torch.equal(b.out[5:], ref) and (b.out[:5] == 5).all()
+
+
+def test_calls_on_no_rows(vxb):
+    e = lambda *s, d=torch.bfloat16: torch.empty(*s, dtype=d, device="cuda")  # noqa: E731
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    vxb.rms_norm(e(0, 64), e(64), e(0, 64))
+    vxb.fp8_product(e(0, 64, d=F8), e(0, 1, d=torch.float32), e(5, 64, d=F8), e(1, 1, d=torch.float32), e(0, 5))
+    q, k, c, pos, f = e(0, 4, 64), e(0, 2, 64), e(3, 16, 2, 64), e(0, d=torch.int64), e(32, d=torch.float32)
+    vxb.rotary(q, pos, f, q)
+    vxb.rotary_append(q, k, k, pos, pos, f, q, c, c)
+    vxb.paged_attention(q, c, c, i(0, 0).view(1, 2), i(0, 0), i(9), q)
+    one, table = randn(1, 1, 4, 64, dtype=torch.bfloat16), e(0, 2, d=torch.int32)
+    out = torch.full_like(one, 5.0)
+    vxb.paged_attention(one, c, c, table, i(0), i(), out)  # no sequences: every row is outside
+    torch.cuda.synchronize()
+    assert (out == 5).all()
 
 
 @pytest.mark.parametrize("q_len", [1, 200])
