@@ -327,9 +327,10 @@ VXB_API int vxb_convt(const void* w, int w_type, int Cin, int Cout, int s, const
  * be NULL, sum may be x or residual; w [C] of `type` or F32.  y is of `type`
  * (y_scale NULL; y may be x), or with y_type E4M3 codes with y_scale
  * [N][ceil(C / 128)]: per row and 128 channels scale = max|y| / 448 and code
- * = e4m3(y / scale), the operand form of vxb_fp8_product (a block whose scale
- * would be below fp32's normal range is zeros with scale 0).  Sums and the
- * norm are fp32 of the unrounded h.  1 <= C <= 32768. */
+ * = e4m3(y / scale), the quotient within an fp32 ulp, the operand form of
+ * vxb_fp8_product (a block whose scale would be below fp32's normal range is
+ * zeros with scale 0).  Sums and the norm are fp32 of the unrounded h: a row
+ * whose sum of squares leaves fp32's range is not normalised.  1 <= C <= 32768. */
 VXB_API int vxb_rms_norm(int type, int64_t N, int C, const void* x, int64_t x_stride, const void* residual,
                          int64_t residual_stride, void* sum, int64_t sum_stride, int w_type, const void* w, float eps,
                          int y_type, void* y, int64_t y_stride, float* y_scale, int64_t scale_stride, void* stream);

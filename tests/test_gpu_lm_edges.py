@@ -1,0 +1,47 @@
+"""The language-model operators at the edges of what their documentation allows:
+values, streams and tensors that the shapes of test_gpu_lm_ops.py do not bring.
+"""
+import pytest
+import torch
+
+from test_gpu_lm_ops import F8, U, Batch, close, codes, half_step, product_ref, randn, vxb  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- rms norm --
+
+@pytest.mark.parametrize("C", [4096, 1000, 77])
+def test_rms_norm_codes_are_the_rounded_quotients(vxb, C):  # noqa: F811
+    """scale = max|y| / 448 (by the rounded 1 / 448, as torch does it: bit for bit) and code = e4m3(y / scale) of
+    the fp32 output y, where a quotient is off by two roundings of 2^-24 at most, and by one more here (blocks of size 2^-60 to 2^60, so that no quotient is special)."""
+    kb = -(-C // 128)
+    x = randn(1, 200, C)
+    w = (randn(2, C) * 2.0 ** torch.linspace(-60, 60, kb, device="cuda").repeat_interleave(128)[:C]).contiguous()
+    y = torch.empty_like(x)
+    vxb.rms_norm(x, w, y)
+    q, s = torch.empty(200, C, dtype=F8, device="cuda"), torch.empty(200, kb, device="cuda")
+    vxb.rms_norm(x, w, q, y_scale=s)
+    top = torch.nn.functional.pad(y, (0, kb * 128 - C)).view(200, kb, 128).abs().amax(2)
+    assert torch.equal(s, top / 448)
+    by = s.repeat_interleave(128, 1)[:, :C]
+    quotient = y.double() / by.double()
+    lo, hi = ((quotient * (1 + d)).float().to(F8).view(torch.uint8) for d in (-(2.0 ** -23), 2.0 ** -23))
+    got = q.view(torch.uint8)
+    assert ((got == lo) | (got == hi)).all()
+
+
+def test_rms_norm_codes_of_the_largest_values(vxb):  # noqa: F811
+    """Blocks whose maximum lies above 2^126 (8.5e37) keep their codes; a block with an infinity has the
+    scale infinity, zeros for what is finite and NaN for what is not."""
+    x = torch.ones(3, 512, device="cuda")
+    x[:, 1::2] = -1
+    w = torch.ones(512, device="cuda")
+    w[:128], w[128:256], w[256] = 2e38, 8e37, float("inf")
+    y, q, s = torch.empty_like(x), torch.empty(3, 512, dtype=F8, device="cuda"), torch.empty(3, 4, device="cuda")
+    vxb.rms_norm(x, w, y)
+    vxb.rms_norm(x, w, q, y_scale=s)
+    for b in (0, 1, 3):
+        assert torch.equal(q[:, 128 * b: 128 * b + 128].float(), 448 * x[:, :128])
+        assert torch.equal(s[:, b], y[:, 128 * b] / 448)
+    assert torch.isinf(s[:, 2]).all() and torch.isnan(q[:, 256].float()).all() and not q[:, 257:384].float().any()

@@ -3,7 +3,7 @@
 //   h = x (+ residual)                        (fp32; also stored, rounded to x's type)
 //   y = h / sqrt(mean(h^2) + eps) * w
 //   out = y in x's type, or e4m3 codes with one fp32 scale per row and block
-//         of 128 channels: scale = max|y| / 448, code = e4m3(y * 448 / max|y|)
+//         of 128 channels: scale = max|y| / 448, code = e4m3(y / scale)
 //
 // HBM bound: per channel one read of x and of the residual, one write of the
 // sum and of the output.  One block per row keeps the row in registers
@@ -101,9 +101,9 @@ __device__ __forceinline__ void store8(T* p, int n, const float* v) {
 // Block of any multiple of 32 threads (<= 1024); NV vectors of 8 channels per
 // thread: C <= 8 * NV * blockDim.x.  VEC: C % 8 == 0 and every row is 16-byte
 // aligned.  The kernel was bound by instructions when it tested every element
-// and divided with rounding: with packed fp32 arithmetic and one approximate
-// division (2 ulp) per block of 128 the 16384 x 4096 bf16 case went from 106
-// to 73 us (6.46 TB/s; 72 us at the measured copy rate).
+// and divided each: with packed fp32 arithmetic and one reciprocal per block of
+// 128 the 16384 x 4096 bf16 case went from 106 to 73 us in a graph (6.45 TB/s; 80
+// us, 5.9 TB/s, a call among others; 72 us at the measured copy rate).
 template <typename T, int NV, bool VEC, bool RES, bool Q8>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
     __shared__ float part[32];
@@ -187,14 +187,19 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
         for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         // A block whose scale would not be a normal fp32 number is all zeros.
         const bool zero = top < kE4m3Max * 1.17549435e-38f;
-        const float inv = zero ? 0.f : __fdividef(kE4m3Max, top);
+        const float s = zero ? 0.f : top * (1.f / kE4m3Max);
         if (n <= 0) continue;
-        if ((lane & 15) == 0) a.scale[row * a.scale_stride + c / kScaleBlock] = zero ? 0.f : top * (1.f / kE4m3Max);
+        if ((lane & 15) == 0) a.scale[row * a.scale_stride + c / kScaleBlock] = s;
+        // y / s as the product with the reciprocal, itself rounded once by a Newton step: at most one
+        // ulp from the quotient (correcting that too, two packed FMAs more, took the case above from
+        // 73.1 to 75.2 us).  (s is below 2^126, where __fdividef ends, and an infinite s gives 0.)
+        float inv = zero ? 0.f : __fdividef(1.f, s);
+        inv = fmaf(fmaf(isinf(s) ? 0.f : -s, inv, 1.f), inv, inv);
+        const float2 iv = make_float2(inv, inv);
         uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.y_stride + c;
         uint32_t code[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const float2 iv = make_float2(inv, inv);
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(fmul2(y[2 * p], iv), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(fmul2(y[2 * p + 1], iv), __NV_SATFINITE, __NV_E4M3);
             code[p] = lo | (hi << 16);
