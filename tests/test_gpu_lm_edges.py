@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("C", [4096, 1000, 77])
 def test_rms_norm_codes_are_the_rounded_quotients(vxb, C):  # noqa: F811
     """scale = max|y| / 448 (by the rounded 1 / 448, as torch does it: bit for bit) and code = e4m3(y / scale) of
-    the fp32 output y, where a quotient is off by two roundings of 2^-24 at most, and by one more here (blocks of size 2^-60 to 2^60, so that no quotient is special)."""
+    the fp32 output y, where a quotient is off by two roundings of 2^-24 at most (blocks of size 2^-60 to 2^60, so that no
+    quotient is special)."""
     kb = -(-C // 128)
     x = randn(1, 200, C)
     w = (randn(2, C) * 2.0 ** torch.linspace(-60, 60, kb, device="cuda").repeat_interleave(128)[:C]).contiguous()
@@ -45,3 +46,39 @@ def test_rms_norm_codes_of_the_largest_values(vxb):  # noqa: F811
         assert torch.equal(q[:, 128 * b: 128 * b + 128].float(), 448 * x[:, :128])
         assert torch.equal(s[:, b], y[:, 128 * b] / 448)
     assert torch.isinf(s[:, 2]).all() and torch.isnan(q[:, 256].float()).all() and not q[:, 257:384].float().any()
+
+
+# ------------------------------------------------------------- fp8 product --
+
+@pytest.mark.parametrize("N", [1, 2, 16, 600])
+def test_norm_and_product_in_turn_in_a_graph(vxb, N):  # noqa: F811
+    """Products right behind the norms that write their operands, with nothing between them but the programmatic
+    launch: new inputs at every replay, bit for bit what calls with a synchronisation between them give."""
+    C, M, layers = 1024, 1024, 6
+    ws = [codes(20 + 10 * i, M, C, 128) for i in range(layers)]
+    gain = [randn(7 + i, C) + 1 for i in range(layers)]
+    x = torch.empty(N, C, device="cuda")
+    q, s = torch.empty(N, C, dtype=F8, device="cuda"), torch.empty(N, C // 128, device="cuda")
+    y = torch.empty(N, M, device="cuda")
+
+    def run(wait):
+        src = x
+        for (w, w_s), g in zip(ws, gain):  # one set of buffers: each pair overwrites what the last one read
+            vxb.rms_norm(src, g, q, y_scale=s)
+            wait()
+            vxb.fp8_product(q, s, w, w_s, y)
+            wait()
+            src = y
+
+    run(lambda: None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(lambda: None)
+    for step in range(8):
+        x.copy_(randn(100 + step, N, C, scale=1.0 + step))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        run(torch.cuda.synchronize)
+        assert torch.equal(got, y)

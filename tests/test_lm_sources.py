@@ -1,0 +1,21 @@
+"""Rules that the language-model kernels keep everywhere, read from their sources:
+no run shows a breach reliably."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "voxcpm-inference_b200", "csrc")
+KERNELS = ["lm_norm.cuh", "lm_rotary.cuh", "fp8_gemm.cuh", "fp8_gemv.cuh", "paged_attn.cuh", "chunk_attn.cuh"]
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+@pytest.mark.parametrize("name", KERNELS)
+def test_operands_are_read_coherently(name):
+    """A launch may start while the kernel that writes its operands still runs: they are not constant for its
+    lifetime, which is what read-only loads ask for."""
+    assert not re.findall(r"__ldg|\.nc\b|__restrict__", source(name))

@@ -155,8 +155,8 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type)
     }
 }
 
-// n consecutive outputs of a row from column c (8 at a time, n a multiple of
-// 8): vectors where the address and the row's end allow it.
+// NV consecutive outputs of a row from column c, 32 bytes at a time: vectors
+// where the address and the row's end allow it.
 template <typename T, int NV>
 __device__ __forceinline__ void store_cols(T* y, int c, int M, const float* bias, const float* acc) {
     constexpr int kVec = 32 / sizeof(T);  // elements of a 32-byte store (a whole sector of the row)
@@ -165,7 +165,7 @@ __device__ __forceinline__ void store_cols(T* y, int c, int M, const float* bias
     for (int i = 0; i < NV; i += kVec) {
         float v[kVec];
 #pragma unroll
-        for (int x = 0; x < kVec; ++x) v[x] = acc[i + x] + (bias && c + i + x < M ? __ldg(bias + c + i + x) : 0.f);
+        for (int x = 0; x < kVec; ++x) v[x] = acc[i + x] + (bias && c + i + x < M ? bias[c + i + x] : 0.f);
         if (fast && c + i + kVec <= M) {
             uint32_t w[8];
             T* e = reinterpret_cast<T*>(w);
@@ -200,7 +200,7 @@ __device__ __forceinline__ void store_tile(const void* tmap_y, uint8_t* buf, int
 #pragma unroll
             for (int i = 0; i < kE; ++i) {
                 const int col = b + c * kE + i;
-                e[i] = from_float<T>(acc[col] + (args.bias && c0 + col < args.M ? __ldg(args.bias + c0 + col) : 0.f));
+                e[i] = from_float<T>(acc[col] + (args.bias && c0 + col < args.M ? args.bias[c0 + col] : 0.f));
             }
             *reinterpret_cast<uint4*>(buf + lane * 128 + (((c ^ lane) & 7) << 4)) = w;
         }
@@ -340,7 +340,9 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             float acc[NC];
 #pragma unroll
             for (int i = 0; i < NC; ++i) acc[i] = 0.f;
-            auto load = [](const float* p, int kb) { return p ? __ldg(p + kb) : 0.f; };
+            // (no read-only loads here: the kernel before, still running when this one starts, may
+            // have written any operand)
+            auto load = [](const float* p, int kb) { return p ? p[kb] : 0.f; };
             float own = 0.f, col = 0.f, col2 = 0.f;
             if (kb_lo < kb_hi) own = load(own_p, kb_lo), col = load(col_p, kb_lo), col2 = load(col_p2, kb_lo);
             bool ok = true;

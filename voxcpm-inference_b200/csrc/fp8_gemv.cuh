@@ -7,7 +7,8 @@
 // each of their rows (neighbouring lanes, neighbouring bytes), converts them
 // exactly (e4m3 -> f16 -> f32) and adds x * w in fp32; a lane's 16 codes lie in
 // one block of 128, so their sum is scaled once.  Lanes are added at the end in
-// a fixed order.  (1 x 1024 -> 4096: 2.4 us against 4.5; 1 x 4096 -> 4096 5.2
+// a fixed order.  Every operand may be what the kernel before wrote while this
+// one was already resident, so none is read through the read-only path.  (1 x 1024 -> 4096: 2.4 us against 4.5; 1 x 4096 -> 4096 5.2
 // against 6.7; 2 x 1024 -> 4096 3.1 against 4.5.  Longer rows or more weights
 // keep the loads of a warp too few: 1 x 8192 -> 8192 19.0 against 16.9, and four
 // tokens make its arithmetic count: 4 x 4096 -> 4096 11.6 against 6.8.)
@@ -33,6 +34,15 @@ __device__ __forceinline__ void e4m3x16(uint4 v, float* f) {
         }
 }
 
+// 16 bytes of an operand, in the order of the other volatile instructions (never ahead of
+// the wait for the kernel before).
+__device__ __forceinline__ uint4 ld_v4(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// NT tokens: args.N == NT.
 template <int NT>
 __global__ void __launch_bounds__(kGemvThreads) fp8_gemv_kernel(const uint8_t* x, int64_t x_stride, const uint8_t* w,
                                                                int64_t w_stride, const Fp8GemmArgs args) {
@@ -62,14 +72,13 @@ __global__ void __launch_bounds__(kGemvThreads) fp8_gemv_kernel(const uint8_t* x
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
             wv[r] = __ldcs(reinterpret_cast<const uint4*>(wp[r] + k));
-            sw[r] = __ldg(ws[r] + b);
+            sw[r] = ws[r][b];
         }
         float xf[NT][16], sx[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const bool on = n < args.N;
-            e4m3x16(on ? __ldg(reinterpret_cast<const uint4*>(x + n * x_stride + k)) : make_uint4(0, 0, 0, 0), xf[n]);
-            sx[n] = on ? __ldg(args.xs + n * args.xs_stride + b) : 0.f;
+            e4m3x16(ld_v4(x + n * x_stride + k), xf[n]);
+            sx[n] = args.xs[n * args.xs_stride + b];
         }
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
@@ -91,7 +100,7 @@ __global__ void __launch_bounds__(kGemvThreads) fp8_gemv_kernel(const uint8_t* x
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) acc[r][n] += __shfl_xor_sync(0xffffffffu, acc[r][n], o);
-            if (lane == r * NT + n && m0 + r < args.M && n < args.N)
+            if (lane == r * NT + n && m0 + r < args.M)
                 store_out(args.y, n * args.y_stride + m0 + r, acc[r][n] + (args.bias ? args.bias[m0 + r] : 0.f),
                           args.out_type);
         }
