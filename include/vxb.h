@@ -400,6 +400,19 @@ VXB_API int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, int 
  * current device; -1 if the extents are refused (vxb_last_error). */
 VXB_API int64_t vxb_paged_attention_workspace(int64_t N, int B, int Hq, int Hk, int D, int max_pages, int page_size);
 
+/* Every wait inside these operators' kernels is bounded (2 s).  A kernel whose
+ * wait runs out leaves its output as it was or in part written, records that
+ * in a word of its device and returns, so the stream goes on.  This call waits
+ * for the work on `stream` up to timeout_ms (VXB_ERR_TIMEOUT), reads and clears
+ * the current device's word, and returns VXB_ERR_DEVICE_STATUS if a wait of any
+ * of these operators on the device (any stream) has run out since the last
+ * time.  Not during a capture. */
+VXB_API int vxb_operators_sync(int timeout_ms, void* stream);
+
+/* Makes one such wait run out after limit_us microseconds (1..2000000): the next
+ * vxb_operators_sync reports it (the counterpart of vxb_debug_wait_probe). */
+VXB_API int vxb_debug_operators_wait_probe(int limit_us, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,3 +82,33 @@ def test_norm_and_product_in_turn_in_a_graph(vxb, N):  # noqa: F811
         got = y.clone()
         run(torch.cuda.synchronize)
         assert torch.equal(got, y)
+
+
+# ------------------------------------------------------------ failed waits --
+
+def test_expired_wait_is_reported_once_and_operators_go_on(vxb):  # noqa: F811
+    x, xs = codes(1, 9, 1024, 1)
+    w, ws = codes(5, 640, 1024, 128)
+    a, y = (torch.empty(9, 640, device="cuda") for _ in range(2))
+    vxb.fp8_product(x, xs, w, ws, a)
+    vxb.operators_sync()
+    side = torch.cuda.Stream()
+    vxb.operators_wait_probe(1000, stream=side)
+    vxb.fp8_product(x, xs, w, ws, y, stream=side)
+    with pytest.raises(vxb.VxbError) as e:
+        vxb.operators_sync(5000, stream=side)
+    assert e.value.code == vxb.ERR_DEVICE_STATUS and "wait" in str(e.value)
+    vxb.operators_sync(stream=side)  # read and cleared
+    vxb.operators_sync()
+    assert torch.equal(a, y)
+
+
+def test_operators_sync_gives_up_at_its_timeout(vxb):  # noqa: F811
+    vxb.operators_wait_probe(300000)
+    with pytest.raises(vxb.VxbError) as e:
+        vxb.operators_sync(10)
+    assert e.value.code == vxb.ERR_TIMEOUT
+    with pytest.raises(vxb.VxbError) as e:
+        vxb.operators_sync()
+    assert e.value.code == vxb.ERR_DEVICE_STATUS
+    vxb.operators_sync()

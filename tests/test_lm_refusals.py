@@ -155,3 +155,9 @@ def test_entry_arguments_match_their_signatures():
                     ("paged_attention", ATTN)):
         assert len(a) == len(vxb.SIGNATURES["vxb_" + name][1])
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_operators_sync_refuses():
+    assert vxb.lib().vxb_operators_sync(-1, None) == vxb.ERR_INVALID_ARGUMENT
+    for bad in (0, -3, 2000001):
+        assert vxb.lib().vxb_debug_operators_wait_probe(bad, None) == vxb.ERR_INVALID_ARGUMENT

@@ -19,3 +19,13 @@ def test_operands_are_read_coherently(name):
     """A launch may start while the kernel that writes its operands still runs: they are not constant for its
     lifetime, which is what read-only loads ask for."""
     assert not re.findall(r"__ldg|\.nc\b|__restrict__", source(name))
+
+
+@pytest.mark.parametrize("name", KERNELS)
+def test_waits_that_run_out_are_recorded(name):
+    """Every wait is bounded and goes through op_wait, and every kernel that waits records a failure at its end."""
+    s = source(name)
+    assert not re.findall(r"\bmbar_wait(?:_for)?\s*\(|\bmbar_try_wait\s*\(", s)
+    kernels = re.split(r"\b__global__\b", s)[1:]
+    for k in kernels:
+        assert ("op_wait(" in k) == ("record_abort(" in k)

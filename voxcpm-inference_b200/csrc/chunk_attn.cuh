@@ -34,6 +34,7 @@
 #include <cuda.h>
 
 #include "fp8_gemm.cuh"
+#include "op_status.cuh"
 #include "paged_attn.cuh"
 
 namespace vxb {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                 int pg = -1;
                 if (bx < boxes && j < key_hi) pg = table[j >> a.page_shift];
                 if (lane == 0) {
-                    ok = mbar_wait(&empty[slot], ((i / R) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty);
+                    ok = op_wait(&empty[slot], ((i / R) & 1) ^ 1, abort_flag, kErrWaitEmpty);
                     if (ok) mbar_arrive_expect_tx(&full[slot], Cfg::kTileBytes);
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             const uint32_t leader = lane == 0;
             const uint32_t q_addr = smem_u32(sq) >> 4, ring_addr = smem_u32(ring) >> 4;
             auto wait = [&](uint64_t* bar, int parity, int code) {
-                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, nullptr, code)) != 0;
+                return __all_sync(0xffffffffu, op_wait(bar, parity, abort_flag, code)) != 0;
             };
             auto scores = [&](int i, int slot) {  // S_i = Q_i K^T
                 const uint32_t qa = kLow | (q_addr + i * (H * 16384 / 16));
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
         bool ok = true;
         for (int i = 0; i < 2 * steps; ++i) {
             const int slot = i % R;
-            ok = mbar_wait(&full[slot], (i / R) & 1, abort_flag, nullptr, kErrWaitFull);
+            ok = op_wait(&full[slot], (i / R) & 1, abort_flag, kErrWaitFull);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if ((i & 1) && !even(my_lo + (i >> 1))) {
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             const int step = my_lo + j;
             const uint32_t there = __ballot_sync(0xffffffffu, here) & 0xffu;
             here = j + 1 < n && present(step + 1);
-            ok = mbar_wait(&s_full[i], j & 1, abort_flag, nullptr, kErrWaitAccum);
+            ok = op_wait(&s_full[i], j & 1, abort_flag, kErrWaitAccum);
             ok = __all_sync(0xffffffffu, ok && !*abort_flag);
             if (!ok) break;
             tc_fence_after();
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
                 m = mn;
                 l *= f;
                 if (j > 0) {
-                    ok = mbar_wait(&o_done[i], (j - 1) & 1, abort_flag, nullptr, kErrWaitAccum);
+                    ok = op_wait(&o_done[i], (j - 1) & 1, abort_flag, kErrWaitAccum);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -475,8 +476,8 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             l += (sum.x + sum.y) + (sum2.x + sum2.y);
         }
         if (n > 0 && ok) {
-            ok = mbar_wait(&o_done[i], (n - 1) & 1, abort_flag, nullptr, kErrWaitAccum);
-            ok = ok && mbar_wait(end_bar, 0, abort_flag, nullptr, kErrWaitAccum);
+            ok = op_wait(&o_done[i], (n - 1) & 1, abort_flag, kErrWaitAccum);
+            ok = ok && op_wait(end_bar, 0, abort_flag, kErrWaitAccum);
             ok = __all_sync(0xffffffffu, ok && !*abort_flag);
             if (ok) tc_fence_after();
         }
@@ -526,6 +527,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    if (tid == 0) record_abort(abort_flag);
     if (warp == 9) tmem_dealloc(tmem, 512);
 }
 

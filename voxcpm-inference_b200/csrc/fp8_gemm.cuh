@@ -36,6 +36,7 @@
 #include <cuda.h>
 
 #include "lm_norm.cuh"
+#include "op_status.cuh"
 
 namespace vxb {
 
@@ -114,6 +115,13 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t saddr, uint32_t rank
         : "r"(saddr), "r"(rank)
         : "memory");
     return v;
+}
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t saddr, uint32_t rank, uint32_t v) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.u32 [a], %2;\n}\n" ::"r"(
+                     saddr),
+                 "r"(rank), "r"(v)
+                 : "memory");
 }
 
 constexpr int kMaxSplit = 8;  // blocks of a cluster
@@ -271,7 +279,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                 const int c0 = static_cast<int>(tile / args.row_tiles) * BN;
                 for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
                     const int st = it % S;
-                    if (!mbar_wait(&empty_bar[st], ((it / S) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty)) break;
+                    if (!op_wait(&empty_bar[st], ((it / S) & 1) ^ 1, abort_flag, kErrWaitEmpty)) break;
                     uint8_t* dst = stages + st * Cfg::kStageBytes;
                     mbar_arrive_expect_tx(&full_bar[st], Cfg::kStageBytes);
                     tma_load_2d(dst, &tmap_a, &full_bar[st], kb * 128, r0);
@@ -294,8 +302,8 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
             for (int64_t tile = tile0; tile < args.tiles && ok; tile += tile_step) {
                 for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
                     const int st = it % S, buf = it & 1;
-                    if (!mbar_wait(&full_bar[st], (it / S) & 1, abort_flag, nullptr, kErrWaitFull) ||
-                        !mbar_wait(&tempty_bar[buf], ((it >> 1) & 1) ^ 1, abort_flag, nullptr, kErrWaitAccum)) {
+                    if (!op_wait(&full_bar[st], (it / S) & 1, abort_flag, kErrWaitFull) ||
+                        !op_wait(&tempty_bar[buf], ((it >> 1) & 1) ^ 1, abort_flag, kErrWaitAccum)) {
                         ok = false;
                         break;
                     }
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
                     col_n = load(col_p, kb + 1);
                     col2_n = load(col_p2, kb + 1);
                 }
-                ok = mbar_wait(&tfull_bar[buf], (it >> 1) & 1, abort_flag, nullptr, kErrWaitAccum);
+                ok = op_wait(&tfull_bar[buf], (it >> 1) & 1, abort_flag, kErrWaitAccum);
                 ok = __all_sync(0xffffffffu, ok && !*abort_flag);
                 if (!ok) break;
                 tc_fence_after();
@@ -428,7 +436,11 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
     if (Cfg::kTmaOut && args.tma_out && warp >= 4 && lane == 0) bulk_wait_all();  // stores done before the staging goes
     if (Cfg::kSplits && split > 1) {
         __syncwarp();
-        cluster_arrive_wait();  // every rank's partial sums are written
+        if (*abort_flag && lane == 0)  // a rank that gave up takes the others with it
+            for (int p = 0; p < split; ++p)
+                st_cluster_u32(smem_u32(const_cast<const int*>(abort_flag)), p, *abort_flag);
+        __syncwarp();
+        cluster_arrive_wait();  // every rank's partial sums are written, or every rank's flag is set
         if (!*abort_flag && tile0 < args.tiles) {
             const int r0 = static_cast<int>(tile0 % args.row_tiles) * 128;
             const int64_t c0 = tile0 / args.row_tiles * BN;
@@ -460,6 +472,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, WROWS>::kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) record_abort(abort_flag);
     if (warp == 1) tmem_dealloc(tmem_base, Cfg::kTmemCols);
 }
 

@@ -27,6 +27,9 @@ EncodeTiledFn encode_fn();
 // Streaming multiprocessors of device `dev`.
 int num_sms(int dev);
 
+// Waits for a stream's work up to timeout_ms (VXB_ERR_TIMEOUT).
+int wait_stream(cudaStream_t s, int timeout_ms);
+
 #define CUDA_TRY(expr)                                                                              \
     do {                                                                                            \
         cudaError_t e_ = (expr);                                                                    \

@@ -556,3 +556,32 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
                                     : launch_attn<__nv_bfloat16>(a, p, dev, st);
     });
 }
+
+// ------------------------------------------------------------ failed waits --
+
+extern "C" int vxb_operators_sync(int timeout_ms, void* stream) {
+    return guarded([&]() -> int {
+        if (timeout_ms < 0) return bad("operators_sync", "the timeout must not be negative");
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        int code = 0;
+        if (int rc = wait_stream(st, timeout_ms)) return rc;
+        CUDA_TRY(cudaMemcpyFromSymbolAsync(&code, g_op_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+        CUDA_TRY(cudaStreamSynchronize(st));
+        if (!code) return VXB_OK;
+        const int none = 0;
+        CUDA_TRY(cudaMemcpyToSymbolAsync(g_op_status, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+        CUDA_TRY(cudaStreamSynchronize(st));
+        return fail(VXB_ERR_DEVICE_STATUS, "a language-model operator's bounded wait failed (code " +
+                                               std::to_string(code) + "): its output is not valid");
+    });
+}
+
+extern "C" int vxb_debug_operators_wait_probe(int limit_us, void* stream) {
+    return guarded([&]() -> int {
+        if (limit_us < 1 || limit_us > 2000000) return bad("operators_wait_probe", "bad limit");
+        op_wait_probe_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<unsigned long long>(limit_us) *
+                                                                              1000ull);
+        CUDA_TRY(cudaGetLastError());
+        return VXB_OK;
+    });
+}

@@ -37,6 +37,7 @@
 #include <cuda.h>
 
 #include "lm_norm.cuh"
+#include "op_status.cuh"
 
 namespace vxb {
 
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
             for (int step = first; step < min(first + per, my_hi); ++step) {
                 const int i = step - my_lo, slot = i % S;
                 int pg = __shfl_sync(0xffffffffu, cur, ((step - first) * bps + bx) & 31);
-                ok = mbar_wait(&empty[slot], ((i / S) & 1) ^ 1, abort_flag, nullptr, kErrWaitEmpty);
+                ok = op_wait(&empty[slot], ((i / S) & 1) ^ 1, abort_flag, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 // bit g: keys 16 g .. 16 g + 15 of the step lie in a page
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
         const int j0 = step * kStep + warp * 16 * KW;  // this warp's keys
         // does every row see all of the warp's keys?
         bool whole = j0 + 16 * KW - 1 <= pos_min && (a.window <= 0 || j0 > pos_max - a.window);
-        ok = mbar_wait(&full[slot], (it / S) & 1, abort_flag, nullptr, kErrWaitFull);
+        ok = op_wait(&full[slot], (it / S) & 1, abort_flag, kErrWaitFull);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         // bit i: key j0 + i lies in no page
@@ -525,7 +526,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(const __grid_co
     }
     if (poison) sh_poison = 1;
     __syncthreads();  // every copy has landed and been read: the ring is free
-    if (*abort_flag) return;
+    if (*abort_flag) {
+        if (tid == 0) record_abort(abort_flag);
+        return;
+    }
 
     // Join the four warps: each leaves its output (rows padded by 4 words: no bank
     // conflicts), maximum and sum; then a thread adds 4 dims of a row.

@@ -83,6 +83,8 @@ SIGNATURES = {
     "vxb_paged_attention": (_i, [_i, _i64, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _vp,
                                  _i64, _i, _vp, _vp, _f, _i, _vp, _i64, _i64, _vp, _i64, _vp]),
     "vxb_paged_attention_workspace": (_i64, [_i64, _i, _i, _i, _i, _i, _i]),
+    "vxb_operators_sync": (_i, [_i, _vp]),
+    "vxb_debug_operators_wait_probe": (_i, [_i, _vp]),
 }
 
 
@@ -590,3 +592,16 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale: 
     one is taken from torch's allocator on the call's stream."""
     (_native_module or _native()).paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale, window,
                                                   workspace, stream)
+
+
+def operators_sync(timeout_ms: int = 60000, stream=None):
+    """Waits for the work on `stream` (None: the current one) and raises
+    VxbError(ERR_DEVICE_STATUS) if a bounded wait inside one of these operators
+    has run out on the current device since the last call: what it was writing
+    is not valid."""
+    check(lib().vxb_operators_sync(timeout_ms, _stream(stream)))
+
+
+def operators_wait_probe(limit_us: int, stream=None):
+    """Makes a bounded wait of these operators run out after limit_us microseconds."""
+    check(lib().vxb_debug_operators_wait_probe(limit_us, _stream(stream)))
