@@ -29,3 +29,11 @@ def test_waits_that_run_out_are_recorded(name):
     kernels = re.split(r"\b__global__\b", s)[1:]
     for k in kernels:
         assert ("op_wait(" in k) == ("record_abort(" in k)
+
+
+@pytest.mark.parametrize("name", KERNELS + ["gemm.cuh", "resunit.cuh", "convt_tm.cuh", "encoder.cuh"])
+def test_tensor_memory_is_taken_before_dependents_are_released(name):
+    """A dependent may take columns before its own wait: it must not find any that this kernel still asks for."""
+    for k in re.split(r"\b__global__\b", source(name))[1:]:
+        alloc, release = k.find("tmem_alloc("), re.search(r"grid_dep_(?:sync|launch)\(\)", k)
+        assert alloc < 0 or release is None or alloc < release.start()

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
             prefetch_tmap(&tmap_v);
         }
     }
-    grid_dep_sync();
+    grid_dep_wait();
     const AttnTile t = a.B <= kCkSort ? find_long_tile(a, slot, 2 * TT, &sh_tile, reinterpret_cast<int2*>(ring))
                                       : find_tile(a, gridDim.x / heads_y - 1 - slot, 2 * TT, &sh_tile);
     if (t.b < 0) return;
@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kCkThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    grid_dep_launch();  // (the tensor memory is this block's)
     const uint32_t tmem = *tmem_slot;
     // TMEM columns: S (and P) of tile i at 128 i, O of tile i at 256 + 128 i
 

@@ -118,9 +118,14 @@ __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, vo
 // its memory operations are visible; launch_dependents then lets the next
 // kernel be scheduled (issued only after the wait, so at most two grids are
 // in flight).  Without a programmatic prerequisite both are no-ops.
+// A kernel takes its TMEM before it lets the next be scheduled: a dependent
+// that takes columns ahead of its own wait could otherwise hold what a block of
+// this kernel still waits for, and wait for that block's end.
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_sync() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    grid_dep_wait();
+    grid_dep_launch();
 }
 
 // -------------------------------------------------------------------- TMA --
