@@ -112,3 +112,21 @@ def test_operators_sync_gives_up_at_its_timeout(vxb):  # noqa: F811
         vxb.operators_sync()
     assert e.value.code == vxb.ERR_DEVICE_STATUS
     vxb.operators_sync()
+
+
+# --------------------------------------------------------- paged attention --
+
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_attention_non_finite_value_of_no_weight_in_a_part_of_its_own(vxb, q_len):  # noqa: F811
+    """A value that a token sees reaches it whatever its weight, also where the keys are split and the part
+    that holds it is outweighed by more than fp32's range."""
+    b = Batch([q_len], [5000], 16, 2, 128, 64, torch.bfloat16)
+    b.q.fill_(1.0)
+    for j in range(5000 // 64 + 1):
+        b.k[int(b.table[0, j])] = -30.0 if j < 16 else 0.0  # scores of -339 at the first 1024 keys, 0 elsewhere
+    b.v[int(b.table[0, 1]), 3, 1, 7] = float("inf")
+    assert vxb.lib().vxb_paged_attention_workspace(q_len, 1, 16, 2, 128, b.table.shape[1], 64) > 0
+    out = b.run(vxb)
+    bad = torch.zeros(q_len, 16, 128, dtype=torch.bool, device="cuda")
+    bad[:, 8:, 7] = True
+    assert torch.equal(~torch.isfinite(out), bad)

@@ -642,10 +642,13 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     float sum = w[0] + w[1];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // (parts that are empty are not read; one whose weight is only too small for fp32 is, since a
+    // non-finite value in it reaches the row all the same)
+    const uint32_t some[2] = {__ballot_sync(0xffffffffu, lse[0] != kNegInf), __ballot_sync(0xffffffffu, lse[1] != kNegInf)};
 #pragma unroll 4
     for (int s = mine; s < a.splits; s += kWarps) {
         const float f = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
-        if (lane * 4 < a.D && f != 0.f) {
+        if (lane * 4 < a.D && ((s < 32 ? some[0] : some[1]) >> (s & 31) & 1)) {
             const float4 o = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.D + lane * 4);
             v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
         }
