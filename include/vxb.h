@@ -319,7 +319,9 @@ VXB_API int vxb_convt(const void* w, int w_type, int Cin, int Cout, int s, const
  * which holds the codec only.  Strides count elements.  Calls return once
  * their work is enqueued; every launch is on `stream` of the current device,
  * allocates nothing and may be captured into a graph.  Work on zero rows is a
- * success without a launch.  Outputs must not overlap inputs unless said. */
+ * success without a launch.  Outputs must not overlap inputs unless said, nor
+ * their own rows: their axes nest, each stride at least the extent of what
+ * lies inside it. */
 
 /* Root-mean-square norm of rows, the residual added first:
  *   h = x (+ residual);  sum = h;  y = h / sqrt(mean(h^2) + eps) * w

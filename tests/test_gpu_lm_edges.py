@@ -130,3 +130,23 @@ def test_attention_non_finite_value_of_no_weight_in_a_part_of_its_own(vxb, q_len
     bad = torch.zeros(q_len, 16, 128, dtype=torch.bool, device="cuda")
     bad[:, 8:, 7] = True
     assert torch.equal(~torch.isfinite(out), bad)
+
+
+def test_outputs_of_any_nesting_and_refused_overlaps(vxb):  # noqa: F811
+    b = Batch([3, 2], [40, 20], 4, 2, 64, 16, torch.bfloat16)
+    ref = b.run(vxb).clone()
+    b.out = torch.full((4, 5, 64), 5.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)  # heads outside
+    assert torch.equal(b.run(vxb), ref)
+    inv, pos = torch.from_numpy(vxb.rotary_frequencies(64)[0]).cuda(), torch.arange(5, device="cuda")
+    plain = torch.empty_like(b.q)
+    vxb.rotary(b.q, pos, inv, plain)
+    outside = torch.empty(4, 5, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    vxb.rotary(b.q, pos, inv, outside)
+    assert torch.equal(plain, outside)
+    for wrong in (torch.empty_like(ref[:1]).expand(5, 4, 64), torch.empty_like(ref[:, :1]).expand(5, 4, 64),
+                  torch.empty(5 * 256, dtype=torch.bfloat16, device="cuda").as_strided((5, 4, 64), (128, 64, 1))):
+        for call in (lambda: vxb.rotary(b.q, pos, inv, wrong),
+                     lambda: vxb.paged_attention(b.q, b.k, b.v, b.table, b.cu, b.kv, wrong)):
+            with pytest.raises(vxb.VxbError) as e:
+                call()
+            assert e.value.code == vxb.ERR_INVALID_ARGUMENT

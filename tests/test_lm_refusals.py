@@ -161,3 +161,17 @@ def test_operators_sync_refuses():
     assert vxb.lib().vxb_operators_sync(-1, None) == vxb.ERR_INVALID_ARGUMENT
     for bad in (0, -3, 2000001):
         assert vxb.lib().vxb_debug_operators_wait_probe(bad, None) == vxb.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("name,base,change", [
+    ("rotary", "ROT", dict(qot=0)), ("rotary", "ROT", dict(qoh=0)), ("rotary", "ROT", dict(qoh=32)),
+    ("rotary", "ROT", dict(qot=192)), ("rotary", "ROT", dict(kot=64)), ("rotary", "ROT", dict(koh=-63)),
+    ("rotary_append", "APPEND", dict(qoh=0)), ("rotary_append", "APPEND", dict(ps=0)),
+    ("rotary_append", "APPEND", dict(ss=64)), ("rotary_append", "APPEND", dict(hs=32)),
+    ("rotary_append", "APPEND", dict(ps=1024)), ("paged_attention", "ATTN", dict(ot=0)),
+    ("paged_attention", "ATTN", dict(oh=0)), ("paged_attention", "ATTN", dict(oh=56)),
+    ("paged_attention", "ATTN", dict(ot=64)), ("paged_attention", "ATTN", dict(ot=2 ** 62, oh=1))])
+def test_outputs_whose_heads_overlap_are_refused(name, base, change):
+    """(Threads would race for one place.)"""
+    assert rc(name, *{**globals()[base], **change}.values()) == vxb.ERR_INVALID_ARGUMENT
+    assert b"overlap" in vxb.lib().vxb_last_error()

@@ -9,6 +9,7 @@
 #include <cmath>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #include "chunk_attn.cuh"
 #include "fp8_gemm.cuh"
@@ -34,6 +35,27 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 int elem_size(int type) { return type == VXB_TYPE_F32 ? 4 : 2; }
 
 bool is_float(int type) { return type == VXB_TYPE_F32 || type == VXB_TYPE_F16 || type == VXB_TYPE_BF16; }
+
+// An output's rows of `width` elements along axes of (extent, stride): does each have memory of
+// its own?  (As axes nest, the next one has to step over the whole of those inside it.)
+struct Axis {
+    int64_t extent, stride;
+};
+bool rows_apart(int64_t width, Axis a, Axis b, Axis c = {1, 0}) {
+    const auto step = [](const Axis& x) {  // (an axis of one element has any stride)
+        return x.extent < 2 ? static_cast<__int128>(0) : x.stride < 0 ? -static_cast<__int128>(x.stride) : x.stride;
+    };
+    if (step(b) < step(a)) std::swap(a, b);
+    if (step(c) < step(b)) std::swap(b, c);
+    if (step(b) < step(a)) std::swap(a, b);
+    __int128 span = width;
+    for (const Axis& x : {a, b, c}) {
+        if (x.extent < 2) continue;
+        if (step(x) < span) return false;
+        span += step(x) * (x.extent - 1);
+    }
+    return true;
+}
 
 int this_device(int* dev) {
     CUDA_TRY(cudaGetDevice(dev));
@@ -148,6 +170,12 @@ int run_rotary(const char* op, int type, RotaryArgs a, int interleaved, void* st
         if (!aligned(p, es)) return bad(op, "a pointer is not aligned to its element");
     if (!aligned(a.positions, 8) || !aligned(a.slots, 8) || !aligned(a.inv_freq, 4))
         return bad(op, "positions, slots or frequencies are not aligned to their elements");
+    if (!rows_apart(a.D, {a.N, a.q_out.token}, {a.Hq, a.q_out.head}) ||
+        (a.k_out.p && !rows_apart(a.D, {a.N, a.k_out.token}, {a.Hk, a.k_out.head})) ||
+        (a.k_cache && a.cache_slots > 0 &&
+         !rows_apart(a.D, {a.cache_slots / a.page_size, a.page_stride}, {a.page_size, a.slot_stride},
+                     {a.Hk, a.cache_head})))
+        return bad(op, "heads of an output overlap");
     const int vec = 16 / es;
     const bool v = a.D % vec == 0 && a.R % (2 * vec) == 0 && head_vec(a.q.p, a.q.token, a.q.head, vec) &&
                    head_vec(a.q_out.p, a.q_out.token, a.q_out.head, vec) &&
@@ -524,6 +552,7 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
             return bad(op, "strides of queries and cache must not be negative or beyond 2^38");
         if (!aligned(out, 2) || !aligned(block_table, 4) || !aligned(cu_q, 4) || !aligned(kv_len, 4))
             return bad(op, "a pointer is not aligned to its element");
+        if (!rows_apart(D, {N, o_token}, {Hq, o_head})) return bad(op, "heads of the output overlap");
         int dev = 0;
         if ((rc = this_device(&dev))) return rc;
         AttnArgs a{};
