@@ -150,3 +150,57 @@ def test_outputs_of_any_nesting_and_refused_overlaps(vxb):  # noqa: F811
             with pytest.raises(vxb.VxbError) as e:
                 call()
             assert e.value.code == vxb.ERR_INVALID_ARGUMENT
+
+
+# -------------------------------------------------------------- tensors --
+
+def operator_calls(vxb):  # noqa: F811
+    """(call, its tensors by name, those it writes) of every operator."""
+    bf = torch.bfloat16
+    x, w = randn(1, 4, 256, dtype=bf), randn(2, 256, dtype=bf)
+    x8, xs = codes(3, 4, 256, 1)
+    w8, ws = codes(4, 64, 256, 128)
+    b = Batch([4], [40], 4, 2, 64, 16, bf)
+    pos, slots = torch.arange(4, device="cuda"), torch.arange(4, device="cuda")
+    inv = torch.from_numpy(vxb.rotary_frequencies(64)[0]).cuda()
+    k = randn(5, 4, 2, 64, dtype=bf)
+    e = torch.empty_like
+    return [
+        (vxb.rms_norm, dict(x=x, weight=w, y=e(x), residual=x.clone(), sum_out=e(x)), ("y", "sum_out")),
+        (vxb.rms_norm, dict(x=x, weight=w, y=torch.empty(4, 256, dtype=F8, device="cuda"),
+                            y_scale=torch.empty(4, 2, device="cuda")), ("y", "y_scale")),
+        (vxb.fp8_product, dict(x=x8, x_scale=xs, w=w8, w_scale=ws, y=torch.empty(4, 64, device="cuda"),
+                               bias=torch.zeros(64, device="cuda")), ("y",)),
+        (vxb.rotary, dict(q=b.q, positions=pos, inv_freq=inv, q_out=e(b.q), k=k, k_out=e(k)), ("q_out", "k_out")),
+        (vxb.rotary_append, dict(q=b.q, k=k, v=k.clone(), positions=pos, slots=slots, inv_freq=inv, q_out=e(b.q),
+                                 k_cache=b.k, v_cache=b.v), ("q_out", "k_cache", "v_cache")),
+        (vxb.paged_attention, dict(q=b.q, k_cache=b.k, v_cache=b.v, block_table=b.table, cu_q=b.cu, kv_len=b.kv,
+                                   out=b.out), ("out",)),
+    ]
+
+
+def test_calls_raise_the_version_of_what_they_write(vxb):  # noqa: F811
+    """autograd refuses a saved tensor that a call has overwritten since."""
+    for call, t, written in operator_calls(vxb):
+        before = {n: v._version for n, v in t.items()}
+        call(**t)
+        for n, v in t.items():
+            assert (v._version > before[n]) == (n in written), (call.__name__, n)
+
+
+def test_calls_refuse_to_lose_a_gradient(vxb):  # noqa: F811
+    """No operator has a backward pass: with gradients on, a tensor that asks for one is refused."""
+    for call, t, _ in operator_calls(vxb):
+        for n, v in t.items():
+            if not v.is_floating_point() or v.dtype == F8:
+                continue
+            with_grad = {**t, n: v.detach().requires_grad_()}
+            with pytest.raises(vxb.VxbError) as e:
+                call(**with_grad)
+            assert e.value.code == vxb.ERR_INVALID_ARGUMENT and "gradient" in str(e.value)
+            with torch.no_grad():
+                call(**with_grad)
+    with torch.inference_mode():  # (its tensors have no versions)
+        for call, t, _ in operator_calls(vxb):
+            call(**t)
+    torch.cuda.synchronize()

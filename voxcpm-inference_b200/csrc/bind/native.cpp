@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -65,7 +66,14 @@ struct Call {
     void on_device(const at::Tensor& t) {
         const int d = t.is_cuda() ? t.get_device() : -1;
         if (d < 0 || (device >= 0 && d != device)) refuse(std::string(op) + ": tensors must be on one CUDA device");
+        if (t.requires_grad() && c10::GradMode::is_enabled())
+            refuse(std::string(op) + ": there is no backward pass, but a tensor asks for a gradient (torch.no_grad())");
         device = d;
+    }
+    // Outputs that the call has written: autograd refuses what it saved of them before.
+    static void wrote(std::initializer_list<const at::Tensor*> outputs) {
+        for (const at::Tensor* t : outputs)
+            if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
     // Checks rank, type and that the last axis is contiguous.
     const at::Tensor& of(int i, const char* what, size_t rank, int type) {
@@ -172,6 +180,7 @@ void rms_norm(Call& c) {
                        r ? row_stride(*r, N, C) : 0, h ? ptr(*h) : nullptr, h ? row_stride(*h, N, C) : 0, type_of(w),
                        ptr(w), eps, type_of(y), ptr(y), row_stride(y, N, C), s ? static_cast<float*>(ptr(*s)) : nullptr,
                        s ? row_stride(*s, N, kb) : 0, d.stream));
+    c.wrote({&y, s, h});
 }
 
 // x, x_scale, w, w_scale, y, bias, stream
@@ -195,6 +204,7 @@ void fp8_product(Call& c) {
                           static_cast<const float*>(ptr(xs)), row_stride(xs, N, kb), ptr(w), row_stride(w, M, pitch),
                           static_cast<const float*>(ptr(ws)), b ? static_cast<const float*>(ptr(*b)) : nullptr,
                           type_of(y), ptr(y), row_stride(y, N, M), d.stream));
+    c.wrote({&y});
 }
 
 // Strides of [N][heads][D]; an axis of one element has whatever stride fits.
@@ -240,6 +250,7 @@ void rotary(Call& c) {
                      checked_int(c.op, 2 * f.size(0)), inter, factor, static_cast<const int64_t*>(ptr(pos)),
                      static_cast<const float*>(ptr(f)), hq.p, hq.token, hq.head, hqo.p, hqo.token, hqo.head, hk.p,
                      hk.token, hk.head, hko.p, hko.token, hko.head, d.stream));
+    c.wrote({&qo, ko});
 }
 
 // The two caches of one shape and one set of strides.
@@ -289,6 +300,7 @@ void rotary_append(Call& c) {
                             hq.head, hqo.p, hqo.token, hqo.head, hk.p, hk.token, hk.head, hv.p, hv.token, hv.head,
                             ptr(*m.k), ptr(*m.v), m.pages, checked_int(c.op, m.page), m.page_stride, m.slot_stride,
                             m.head_stride, d.stream));
+    c.wrote({&qo, m.k, m.v});
 }
 
 // q, k_cache, v_cache, block_table, cu_q, kv_len, out, scale, window, workspace, stream
@@ -332,6 +344,7 @@ void paged_attention(Call& c) {
                               B > 1 ? table.stride(0) : max_pages, mp, static_cast<const int32_t*>(ptr(cu)),
                               static_cast<const int32_t*>(ptr(kv)), static_cast<float>(scale), window, ho.p, ho.token,
                               ho.head, ws ? ptr(*ws) : nullptr, ws ? ws->numel() : 0, d.stream));
+    c.wrote({&out, mine.defined() ? nullptr : ws});
 }
 
 template <void (*F)(Call&), int kArgs>

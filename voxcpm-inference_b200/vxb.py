@@ -503,7 +503,8 @@ def residual_unit(w, w_type: int, C: int, d: int, x, batch: int, T: int, a1, dw,
 # `stream` (a torch stream or a handle; None: the device's current stream), on
 # the tensors' device whichever device is current.  A call that the checks of
 # csrc/bind/native.cpp or the C ABI refuse raises
-# VxbError(ERR_INVALID_ARGUMENT) and enqueues nothing.
+# VxbError(ERR_INVALID_ARGUMENT) and enqueues nothing.  There are no backward
+# passes: with gradients on, a tensor that asks for one is refused.
 
 _native_module = None
 
