@@ -1,11 +1,12 @@
-"""Builds libvxb.so (CUDA kernels + C ABI + C++ host API) for sm_100a and the
-Python module _vxb_native.so (torch tensors to the C ABI), in-tree.
+"""Builds libvxb.so (CUDA kernels + C ABI + C++ host API) for sm_100a and, where
+torch and Python's headers are installed, the Python module _vxb_native.so
+(torch tensors to the C ABI), in-tree.
 
     python voxcpm-inference_b200/build.py [-v]
 
 Objects go to voxcpm-inference_b200/_build/, the libraries to
 voxcpm-inference_b200/lib/.  Only files whose sources (or shared
-headers) changed are recompiled.
+headers, or for the module torch) changed are recompiled.
 """
 from __future__ import annotations
 
@@ -35,7 +36,19 @@ def _sources():
 
 
 def _torch():
-    return importlib.util.find_spec("torch").submodule_search_locations[0]
+    """torch's folder, or None where the Python module cannot be built (a C or C++
+    caller of libvxb.so needs neither torch nor Python's headers)."""
+    spec = importlib.util.find_spec("torch")
+    path = spec.submodule_search_locations[0] if spec else ""
+    needed = [os.path.join(path, "include", "c10", "cuda", "CUDAStream.h"),
+              os.path.join(sysconfig.get_paths()["include"], "Python.h")]
+    return path if all(os.path.exists(f) for f in needed) else None
+
+
+def _made_for(torch):
+    """What the module is compiled against besides this repository's sources."""
+    with open(os.path.join(torch, "version.py")) as f:
+        return sys.version + "\n" + torch + "\n" + f.read()
 
 
 def _headers():
@@ -77,26 +90,34 @@ def build(verbose: bool = False) -> str:
         if _stale(o, s, hdr_mtime):
             jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
                          "-I/usr/local/cuda/include", *INC, "-c", s, "-o", o])
+    torch, bind_jobs = _torch(), []
     bind, bind_obj = os.path.join(CSRC, "bind", "native.cpp"), os.path.join(BUILD, "native.cpp.o")
-    abi = os.path.join(ROOT, "include", "vxb.h")
-    bind_stale = _stale(bind_obj, bind, max(os.path.getmtime(abi), os.path.getmtime(__file__)))
-    if bind_stale:
-        inc = os.path.join(_torch(), "include")
-        jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-I" + inc,
-                     "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
-                     "-I" + sysconfig.get_paths()["include"], "-I/usr/local/cuda/include", *INC, "-c", bind, "-o",
-                     bind_obj])
+    stamp = bind_obj + ".for"
+    if torch is None:
+        print("torch or Python.h not found: libvxb.so only, without the Python module " + os.path.basename(NATIVE),
+              file=sys.stderr)
+    else:
+        inc = os.path.join(torch, "include")
+        abi = os.path.join(ROOT, "include", "vxb.h")
+        same = os.path.exists(stamp) and open(stamp).read() == _made_for(torch)
+        if not same or _stale(bind_obj, bind, max(os.path.getmtime(abi), os.path.getmtime(__file__))):
+            bind_jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-I" + inc,
+                              "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+                              "-I" + sysconfig.get_paths()["include"], "-I/usr/local/cuda/include", *INC, "-c", bind,
+                              "-o", bind_obj])
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
-        for out in ex.map(lambda c: _run(c, verbose), jobs):
+        for out in ex.map(lambda c: _run(c, verbose), jobs + bind_jobs):
             if verbose and out.strip():
                 print(out)
     if jobs or not os.path.exists(LIB):
         _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs, "-lpthread", "-ldl", "-lrt"], verbose)
-    if bind_stale or not os.path.exists(NATIVE):
-        lib = os.path.join(_torch(), "lib")
+    if torch is not None and (bind_jobs or not os.path.exists(NATIVE)):
+        lib = os.path.join(torch, "lib")
         _run(["g++", "-shared", "-o", NATIVE, bind_obj, "-L" + os.path.dirname(LIB), "-lvxb", "-L" + lib,
               "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib],
              verbose)
+        with open(stamp, "w") as f:
+            f.write(_made_for(torch))
     return LIB
 
 
