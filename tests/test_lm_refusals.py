@@ -175,3 +175,9 @@ def test_outputs_whose_heads_overlap_are_refused(name, base, change):
     """(Threads would race for one place.)"""
     assert rc(name, *{**globals()[base], **change}.values()) == vxb.ERR_INVALID_ARGUMENT
     assert b"overlap" in vxb.lib().vxb_last_error()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3e38])
+def test_attention_scale_that_overflows_in_log2_units_is_refused(scale):
+    """(Scores of 0 would become 0 * inf.)"""
+    assert rc("paged_attention", *{**ATTN, "scale": scale}.values()) == vxb.ERR_INVALID_ARGUMENT

@@ -537,7 +537,8 @@ extern "C" int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, i
         if (type != VXB_TYPE_F16 && type != VXB_TYPE_BF16) return bad(op, "the type must be f16 or bf16");
         if (pages < 0 || pages >= (int64_t(1) << 31)) return bad(op, "bad page count");
         if (window < 0) return bad(op, "the window must not be negative");
-        if (std::isnan(scale) || std::isinf(scale)) return bad(op, "the scale must be finite");
+        if (std::isnan(scale) || std::isinf(scale * 1.4426950408889634f))  // (in log2 units)
+            return bad(op, "the scale must be finite and below 2.3e38");
         if (N == 0 || B == 0) return VXB_OK;
         if (!q || !out || !cu_q || !kv_len) return bad(op, "null argument");
         if (max_pages > 0 && (!block_table || (pages > 0 && (!k_cache || !v_cache))))
