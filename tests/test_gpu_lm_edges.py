@@ -4,7 +4,7 @@ values, streams and tensors that the shapes of test_gpu_lm_ops.py do not bring.
 import pytest
 import torch
 
-from test_gpu_lm_ops import F8, U, Batch, close, codes, half_step, product_ref, randn, vxb  # noqa: F401
+from test_gpu_lm_ops import F8, Batch, codes, product_ref, randn, vxb  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -84,6 +84,43 @@ def test_norm_and_product_in_turn_in_a_graph(vxb, N):  # noqa: F811
         assert torch.equal(got, y)
 
 
+PRODUCTS = [  # each way the product is formed: no tensor cores, weights as rows, tokens as rows, K split or not
+    (1, 1024, 4096), (2, 2048, 129), (1, 8192, 8192), (3, 528, 70), (16, 1536, 1000), (31, 4096, 512), (64, 8192, 384),
+    (77, 1536, 1001), (256, 1024, 64), (200, 4096, 1024), (129, 256, 130), (700, 512, 7000), (2500, 384, 2056)]
+
+
+@pytest.mark.parametrize("N,K,M", PRODUCTS)
+def test_fp8_product_error_as_a_whole(vxb, N, K, M):  # noqa: F811
+    """The worst case of a long sum hides errors that matter; taken together, errors are as small as fp32's.
+    A product of a block loses at most 2^-24 of the largest value in each of its 128 additions, and each of the
+    blocks' additions 2^-24 of the sum."""
+    x, xs = codes(1, N, K, 1)
+    w, ws = codes(5, M, K, 128)
+    y = torch.empty(N, M, device="cuda")
+    vxb.fp8_product(x, xs, w, ws, y)
+    ref, _ = product_ref(x, xs, w, ws, None)
+    off = (y.double() - ref).square().mean().sqrt() / ref.square().mean().sqrt()
+    assert float(off) <= (128 + 2 * -(-K // 128)) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("N,K,M", PRODUCTS)
+def test_fp8_product_of_small_integers_is_exact(vxb, N, K, M):  # noqa: F811
+    """Codes -2 .. 2 and scales 1/2, 1, 2: every sum is a multiple of 1/4 below 2^17 (64 blocks of 512 times 4), which
+    fp32 holds, so nothing is rounded."""
+    g = torch.Generator(device="cuda").manual_seed(N + K + M)
+
+    def ints(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=g, device="cuda").float()
+
+    x, w = ints(-2, 3, N, K).to(F8), ints(-2, 3, M, K).to(F8)
+    xs, ws = 2.0 ** ints(-1, 2, N, -(-K // 128)), 2.0 ** ints(-1, 2, -(-M // 128), -(-K // 128))
+    bias = ints(-8, 9, M)
+    y = torch.empty(N, M, device="cuda")
+    vxb.fp8_product(x, xs, w, ws, y, bias=bias)
+    ref, _ = product_ref(x, xs, w, ws, bias)
+    assert torch.equal(y.double(), ref)
+
+
 # ------------------------------------------------------------ failed waits --
 
 def test_expired_wait_is_reported_once_and_operators_go_on(vxb):  # noqa: F811
@@ -130,6 +167,37 @@ def test_attention_non_finite_value_of_no_weight_in_a_part_of_its_own(vxb, q_len
     bad = torch.zeros(q_len, 16, 128, dtype=torch.bool, device="cuda")
     bad[:, 8:, 7] = True
     assert torch.equal(~torch.isfinite(out), bad)
+
+
+@pytest.mark.parametrize("q_len,Hq,Hk,D", [([600] + [1] * 20, 16, 2, 64), ([1] * 9 + [300] + [1] * 9, 8, 8, 128),
+                                           ([60] + [1] * 40, 16, 2, 64), ([1] * 30 + [90, 0, 1], 4, 4, 128)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_attention_of_chunks_and_single_tokens_in_one_call(vxb, q_len, Hq, Hk, D, window):  # noqa: F811
+    """One kernel is chosen for the whole batch, from the average: right for both kinds of sequence on either side
+    of the choice."""
+    g = torch.Generator().manual_seed(len(q_len))
+    kv = [n + int(torch.randint(0, 900, (), generator=g)) for n in q_len]
+    b = Batch(q_len, kv, Hq, Hk, D, 16, torch.bfloat16, window=window, tail=2)
+    b.run(vxb)
+    b.check()
+
+
+@pytest.mark.parametrize("q_len", [1, 3, 100])
+def test_attention_of_broadcast_queries_and_caches(vxb, q_len):  # noqa: F811
+    """Inputs may have strides of 0: one query for all tokens or heads, one key head or page for all."""
+    def changes(b):
+        yield {"q": b.q[:1].expand(q_len, 4, 64)}
+        yield {"q": b.q[:, :1].expand(q_len, 4, 64)}
+        yield {n: getattr(b, n)[:, :, :1].expand(-1, -1, 2, -1) for n in ("k", "v")}
+        yield {n: randn(i, 1, 16, 2, 64, dtype=torch.bfloat16).expand(b.k.shape[0], 16, 2, 64)
+               for i, n in enumerate(("k", "v"))}
+
+    for i in range(4):
+        b, ref = (Batch([q_len], [q_len + 60], 4, 2, 64, 16, torch.bfloat16) for _ in range(2))
+        for n, t in list(changes(b))[i].items():
+            setattr(b, n, t)
+            setattr(ref, n, t.contiguous())
+        assert torch.equal(b.run(vxb), ref.run(vxb))
 
 
 def test_outputs_of_any_nesting_and_refused_overlaps(vxb):  # noqa: F811
