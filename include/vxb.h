@@ -365,7 +365,8 @@ VXB_API int vxb_rotary(int type, int64_t N, int Hq, int Hk, int D, int R, int in
  * k_cache and v_cache [pages][page_size][Hk][D] (one set of strides for both,
  * D contiguous).  A slot outside [0, pages * page_size) -- a padding token's
  * -- is skipped; its q is still rotated.  Slots within the cache must differ
- * from one another: which of two tokens with one slot stays is not defined. */
+ * from one another: which of two tokens with one slot stays is not defined.
+ * (vxb_paged_attention reads fewer kinds of cache than this call fills.) */
 VXB_API int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R, int interleaved, float factor,
                               const int64_t* positions, const int64_t* slots, const float* inv_freq, const void* q,
                               int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token, int64_t qo_head,
@@ -378,19 +379,27 @@ VXB_API int vxb_rotary_append(int type, int64_t N, int Hq, int Hk, int D, int R,
  * q [N][Hq][D] and kv_len[b] cached keys, the new tokens' the last of them;
  * token i stands at p = kv_len - q_len + i and sees keys j <= p, with
  * window > 0 also j > p - window:
- *   out = sum_j softmax_j(scale q . k_j) v_j    (zeros if it sees none)
+ *   out = sum_j softmax_j(scale q . k_j) v_j
+ * (zeros if it sees none, or only keys whose score is -inf)
  * Query head h reads key head h / (Hq / Hk).  Key j lies at page
  * block_table[b][j / page_size], place j % page_size, of k_cache and v_cache
  * [pages][page_size][Hk][D] (one set of strides for both).  A table entry
  * outside [0, pages) makes its keys unseen (a page given back by a sliding
  * window); entries past a sequence's keys are not read, kv_len beyond
  * max_pages * page_size (below 2^30) is cut to it, and values that no token sees, non-finite
- * ones too, have no effect.  Rows of q and out outside every sequence are not
- * touched.  type F16 or BF16; D % 8 == 0, D <= 128; page_size a power of two
+ * ones too, have no effect; a non-finite value that a token sees makes its
+ * output non-finite whatever the weight.  Rows of q and out outside every
+ * sequence are not touched.  type F16 or BF16; D % 8 == 0, D <= 128; page_size a power of two
  * >= 16; q and cache bases and strides multiples of 16 bytes.  `workspace`:
  * vxb_paged_attention_workspace bytes of device memory, 16-byte aligned (0:
  * may be NULL), in use until the call's work on `stream` is done.  Scores, softmax and sums
- * are fp32; the weights are rounded to `type` for the second product. */
+ * are fp32; the weights are rounded to `type` for the second product (half a
+ * step each, beside the output's own rounding).
+ *
+ * One kernel and one split of the keys are chosen for the whole call, from the
+ * average rows of a sequence and the number of sequences.  A long chunk among
+ * single tokens, or one sequence far longer than the others of its batch, is
+ * faster in a call of its own (rows, table rows and lengths as views). */
 VXB_API int vxb_paged_attention(int type, int64_t N, int B, int Hq, int Hk, int D, const void* q, int64_t q_token,
                                 int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages,
                                 int page_size, int64_t page_stride, int64_t slot_stride, int64_t head_stride,

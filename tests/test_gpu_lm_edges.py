@@ -4,7 +4,7 @@ values, streams and tensors that the shapes of test_gpu_lm_ops.py do not bring.
 import pytest
 import torch
 
-from test_gpu_lm_ops import F8, Batch, codes, product_ref, randn, vxb  # noqa: F401
+from test_gpu_lm_ops import F8, Batch, close, codes, product_ref, product_tol, randn, vxb  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -198,6 +198,26 @@ def test_attention_of_broadcast_queries_and_caches(vxb, q_len):  # noqa: F811
             setattr(b, n, t)
             setattr(ref, n, t.contiguous())
         assert torch.equal(b.run(vxb), ref.run(vxb))
+
+
+def test_attention_output_quantised_by_the_caller_for_the_next_product(vxb):  # noqa: F811
+    """The step between attention and output projection that no operator makes, in torch as a caller writes it."""
+    b = Batch([5, 1, 70], [40, 33, 200], 4, 2, 64, 16, torch.bfloat16)
+    o = b.run(vxb)
+    blocks = o.view(76, -1, 128).float()
+    o_scale = blocks.abs().amax(-1).clamp_(min=1e-30) / 448
+    o8 = (blocks / o_scale[..., None]).view(76, -1).to(torch.float8_e4m3fn)
+    w, ws = codes(5, 200, 256, 128)
+    x = torch.empty(76, 200, device="cuda")
+    vxb.fp8_product(o8, o_scale, w, ws, x)
+    ref, mag = product_ref(o8, o_scale, w, ws, None)
+    close(x, ref, product_tol(ref, mag, 256, torch.float32))
+    whole, mag = (o.double().view(76, 256).abs() if i else o.double().view(76, 256) for i in (0, 1))
+    wd = w.float().double() * ws.double().repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)
+    # a code is off by half a step of the value (2^-4) or of the smallest step (2^-10 scales)
+    least = o_scale.double().repeat_interleave(128, 1) * 2.0 ** -10
+    off = (torch.maximum(mag * 2.0 ** -4, least) * (1 + 2.0 ** -10)) @ wd.abs().t()
+    assert ((x.double() - whole @ wd.t()).abs() <= off).all()
 
 
 def test_outputs_of_any_nesting_and_refused_overlaps(vxb):  # noqa: F811

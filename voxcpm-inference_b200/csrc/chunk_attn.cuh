@@ -12,11 +12,14 @@
 // on the other tile; the product with V starts on the first 64 keys' weights.
 //
 // Bound (one B200, 4 chunks of up to 2048 tokens over up to 8192 keys, 32 / 8
-// heads of 128: 428 us, 949 TFLOP/s; 242 us at the measured dense rate): a step
+// heads of 128: 460 us a call among others, 883 TFLOP/s, 419 to 458 us in a graph
+// from rest; 242 us at the measured dense rate): a step
 // of both tiles takes about 4100 clocks, the MMAs 2100 and the exponentials of
 // the special-function unit 2048 of them; a tile's softmax takes 2200, and its
-// hand-over to the MMA warp and back 700.  TMEM has no room for a third score
-// buffer beside two outputs of 128 columns.
+// hand-over to the MMA warp and back 700.  At heads of more than 64 dims TMEM has
+// no room for a third score buffer beside two outputs of 128 columns; at 64 it
+// has, 128 columns stay unused (the same chunks, 16 / 2 heads of 64: 204 us, of
+// which the MMAs' rate asks 61).
 //
 // m is the running maximum only loosely: O and the sum are rescaled when the
 // maximum has grown by more than 2^8 since the last time (P stays below 2^8,

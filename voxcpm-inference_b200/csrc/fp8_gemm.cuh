@@ -24,8 +24,9 @@
 //
 // Bounds and measurements (one B200).  Few tokens: 4 x 1024 -> 4096 4.6 us, a
 // chain of launch, TMA, MMA and join; 1 x 8192 -> 8192 16.9 us, 4.0 TB/s of
-// weights.  Many: 8192 x 4096 -> 8192 293 us (1880 TFLOP/s; the MMAs are busy
-// 45 % of the time): 203 us with the scaled additions left out, 177 us with the
+// weights.  Many: 8192 x 4096 -> 8192 347 to 353 us a call among others (1570
+// TFLOP/s), 293 to 323 us in a graph from rest (1700 to 1880; the MMAs are busy
+// 45 % of the time); of 293, 203 us with the scaled additions left out, 177 us with the
 // MMAs free-running, and 992 W at 1640 MHz when it runs on (334 us).
 //
 // Warp roles: warp 0 lane 0 issues TMA loads, warp 1 owns TMEM and issues the

@@ -8,10 +8,13 @@
 // exactly (e4m3 -> f16 -> f32) and adds x * w in fp32; a lane's 16 codes lie in
 // one block of 128, so their sum is scaled once.  Lanes are added at the end in
 // a fixed order.  Every operand may be what the kernel before wrote while this
-// one was already resident, so none is read through the read-only path.  (1 x 1024 -> 4096: 2.4 us against 4.5; 1 x 4096 -> 4096 5.2
-// against 6.7; 2 x 1024 -> 4096 3.1 against 4.5.  Longer rows or more weights
-// keep the loads of a warp too few: 1 x 8192 -> 8192 19.0 against 16.9, and four
-// tokens make its arithmetic count: 4 x 4096 -> 4096 11.6 against 6.8.)
+// one was already resident, so none is read through the read-only path.
+//
+// In a graph, against the tensor path: 1 x 1024 -> 4096 2.3 us against 4.5; 1 x
+// 4096 -> 4096 5.0 against 6.7; 2 x 1024 -> 4096 2.9 against 4.5.  Longer rows or
+// more weights keep the loads of a warp too few: 1 x 8192 -> 8192 19.0 against
+// 16.9, and four tokens make its arithmetic count: 4 x 4096 -> 4096 11.6 against
+// 6.8.
 #pragma once
 
 #include "fp8_gemm.cuh"

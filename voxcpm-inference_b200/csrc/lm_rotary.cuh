@@ -13,7 +13,7 @@
 // HBM bound: q, k, v read and written once.  A block computes its tokens'
 // sines and cosines once into shared memory, for all heads; small blocks (128
 // threads, 4 tokens) so that others move data meanwhile (16381 tokens of 32 + 16
-// heads of 128: 68 us, 5.9 TB/s; 256 threads and 8 tokens with four vectors in
+// heads of 128: 68 us, 5.9 TB/s, in a graph, 71 us a call among others; 256 threads and 8 tokens with four vectors in
 // flight a thread 76 us, with two 69 us, 2 tokens 91 us).  Then every thread
 // moves 16-byte vectors (VEC elements; element by element where a stride or an
 // extent does not allow it).

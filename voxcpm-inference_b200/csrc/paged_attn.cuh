@@ -25,7 +25,9 @@
 // Measured (one B200, 6.55 TB/s copy rate): one token after 131072 keys, 32 / 8
 // heads of 128: 90 us, 5.9 TB/s; 256 tokens after 1 to 2048 keys, 16 / 2 heads of
 // 64: 32 us (19.6 us of bytes; 6.0 to 6.5 TB/s from 8 to 20 us after the start,
-// then the longest sequences' blocks end).  Steps of 128 keys at 64 dims (39 us
+// then the longest sequences' blocks end).  A sequence far longer than the rest
+// of a large batch is not split: 159 of 300 keys and one of 65536, 16 / 2 heads of
+// 64, take 395 us, 27 us in two calls.  Steps of 128 keys at 64 dims (39 us
 // with 64: the per-step overhead of a warp, not its loads, fills the time), 64 KB
 // of ring there so that three blocks share an SM (two with 96 KB: 42 us).
 //
