@@ -417,7 +417,7 @@ VXB_API int64_t vxb_paged_attention_workspace(int64_t N, int B, int Hq, int Hk, 
  * for the work on `stream` up to timeout_ms (VXB_ERR_TIMEOUT), reads and clears
  * the current device's word, and returns VXB_ERR_DEVICE_STATUS if a wait of any
  * of these operators on the device (any stream) has run out since the last
- * time.  Not during a capture. */
+ * time.  A stream that is being captured is refused. */
 VXB_API int vxb_operators_sync(int timeout_ms, void* stream);
 
 /* Makes one such wait run out after limit_us microseconds (1..2000000): the next

@@ -140,6 +140,22 @@ def test_expired_wait_is_reported_once_and_operators_go_on(vxb):  # noqa: F811
     assert torch.equal(a, y)
 
 
+def test_operators_sync_leaves_a_capture_alone(vxb):  # noqa: F811
+    x, w = randn(1, 4, 256), torch.ones(256, device="cuda")
+    a, y = torch.empty_like(x), torch.empty_like(x)
+    vxb.rms_norm(x, w, a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        vxb.rms_norm(x, w, y)
+        with pytest.raises(vxb.VxbError) as e:
+            vxb.operators_sync()
+    assert e.value.code == vxb.ERR_INVALID_ARGUMENT
+    graph.replay()
+    vxb.operators_sync()
+    assert torch.equal(a, y)
+
+
 def test_operators_sync_gives_up_at_its_timeout(vxb):  # noqa: F811
     vxb.operators_wait_probe(300000)
     with pytest.raises(vxb.VxbError) as e:

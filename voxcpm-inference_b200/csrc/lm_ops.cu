@@ -594,6 +594,9 @@ extern "C" int vxb_operators_sync(int timeout_ms, void* stream) {
         if (timeout_ms < 0) return bad("operators_sync", "the timeout must not be negative");
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         int code = 0;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        CUDA_TRY(cudaStreamIsCapturing(st, &capture));
+        if (capture != cudaStreamCaptureStatusNone) return bad("operators_sync", "the stream is being captured");
         if (int rc = wait_stream(st, timeout_ms)) return rc;
         CUDA_TRY(cudaMemcpyFromSymbolAsync(&code, g_op_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
         CUDA_TRY(cudaStreamSynchronize(st));
