@@ -343,7 +343,7 @@ VXB_API int vxb_rms_norm(int type, int64_t N, int C, const void* x, int64_t x_st
  * multiples of 16 bytes); x_scale [N][ceil(K / 128)] (row stride given),
  * w_scale [ceil(M / 128)][ceil(K / 128)] contiguous; bias fp32 [M] or NULL;
  * y [N][M] F32, F16 or BF16.  Products of a block are summed on the tensor
- * cores, blocks in fp32.  Any N and M, 16 <= K <= 2^24. */
+ * cores, blocks in fp32.  Any N, M >= 1, 16 <= K <= 2^24. */
 VXB_API int vxb_fp8_product(int64_t N, int K, int M, const void* x, int64_t x_stride, const float* x_scale,
                             int64_t x_scale_stride, const void* w, int64_t w_stride, const float* w_scale,
                             const float* bias, int y_type, void* y, int64_t y_stride, void* stream);

@@ -181,3 +181,11 @@ def test_outputs_whose_heads_overlap_are_refused(name, base, change):
 def test_attention_scale_that_overflows_in_log2_units_is_refused(scale):
     """(Scores of 0 would become 0 * inf.)"""
     assert rc("paged_attention", *{**ATTN, "scale": scale}.values()) == vxb.ERR_INVALID_ARGUMENT
+
+
+def test_wrappers_refuse_lazily_negated_views():
+    """Their memory holds the values with the other sign."""
+    x, w, y = torch.zeros(4, 256), torch.zeros(256), torch.zeros(4, 256)
+    for a in ((torch._neg_view(x), w, y), (x, torch._neg_view(w), y), (x, w, torch._neg_view(y))):
+        with pytest.raises(vxb.VxbError, match="negated"):
+            vxb.rms_norm(*a)

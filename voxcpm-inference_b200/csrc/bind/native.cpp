@@ -82,6 +82,7 @@ struct Call {
             refuse(std::string(op) + ": " + what + ": expected " + std::to_string(rank) + " axes, got " +
                    shape_text(t.sizes()));
         if (type_of(t) != type) refuse(std::string(op) + ": " + what + ": wrong type");
+        if (t.is_neg()) refuse(std::string(op) + ": " + what + ": a lazily negated view (resolve_neg it)");
         if (t.size(rank - 1) > 1 && t.stride(rank - 1) != 1)
             refuse(std::string(op) + ": " + what + ": the last axis must be contiguous");
         return t;
